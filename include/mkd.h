@@ -557,6 +557,120 @@ int mkd_selfcheck_bf16_round(unsigned long long* mismatches, void* stream);
 int mkd_qwen3_layer_kernel_status(const mkd_qwen3_model* m, int B, const void* workspace,
                                   size_t workspace_bytes, int* used, int* barrier_timeout);
 
+/* ---------------------------------------------------------------------------
+ * Serving many samples of a few prompts on a paged KV cache (no counterparts
+ * in the reference, whose attention_block_tkg appends one row per sequence and
+ * reads a shared prompt once per sequence).  Paged caches here are
+ * [num_blocks, block_len, nkv, d] with any block / row / head strides in
+ * elements (d contiguous), bf16 or e4m3 codes (kv_format MKD_KV_FP8, the
+ * format of mkd_attention_args); d is 64 or 128.
+ *
+ * mkd_kv_append_rope: T new tokens' heads, in fp32 arithmetic,
+ *   q, k: x <- x * rsqrt(mean(x^2) + eps) * norm     (where the norm is given)
+ *   q, k: the first `rot` elements rotated by row positions[t] of cos / sin
+ *         (halves layout: i pairs with i + rot / 2; the rest pass through)
+ * then q rounded to bf16 into q_out, k and v stored at cache row slots[t] =
+ * block * block_len + row: bf16, or e4m3(clip(x * k_scale, +-240)) (v_scale
+ * for v), one rounding from fp32.  A slot outside the pool stores nothing; a
+ * position outside the tables stores nothing and gives a zero q row.  Two
+ * tokens with one slot leave that row undefined (a mix of the two).  q_out may
+ * be q.  T = 0 does nothing.  Rows start on multiples of 4 elements, table
+ * rows and norms too.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  const void *q, *k, *v;       /* [T, nq, d], [T, nkv, d], [T, nkv, d] in x_dtype */
+  int x_dtype;                 /* MKD_DT_*                                       */
+  long long q_stride[2], k_stride[2], v_stride[2]; /* token, head (elements)     */
+  void* q_out;                 /* [T, nq, d] bf16                                */
+  long long q_out_stride[2];
+  const void *q_norm, *k_norm; /* [d] bf16 or NULL                               */
+  float eps;
+  const float *cos, *sin;      /* [table_rows, rot / 2] fp32, or NULL: no rotation */
+  int table_rows, rot;         /* rot a multiple of 8, at most d                 */
+  const void* positions;       /* [T] int32, or int64 with positions_i64; with cos */
+  int positions_i64;
+  void *k_cache, *v_cache;
+  long long k_cache_stride[3], v_cache_stride[3]; /* block, row, head (elements) */
+  int num_blocks, block_len;   /* num_blocks * block_len < 2^31                  */
+  int kv_format;               /* 0 or MKD_KV_FP8                                */
+  const float *k_scale, *v_scale; /* one fp32 value each in device memory (FP8)  */
+  const void* slots;           /* [T] int32, or int64 with slots_i64             */
+  int slots_i64;
+  int T, nq, nkv, d;
+} mkd_kv_append_args;
+int mkd_kv_append_rope(const mkd_kv_append_args* args, void* stream);
+
+/* mkd_attention_shared_prefix: decode attention of B sequences with s_tkg new
+ * tokens each (1 .. 8, already in the cache), q [B, s_tkg, nq, d] bf16 rotated.
+ * Group g's sequences prefix_starts[g] .. prefix_starts[g + 1] - 1 (ascending;
+ * sequences in no group have no prefix) share the prefix_lens[g] positions of
+ * prefix_tables[g]; sequence b then has lens[b] positions of its own in
+ * tables[b], its new tokens last: new token i sees the whole prefix and own
+ * positions 0 .. lens[b] - s_tkg + i.  Position t of a table is row t %
+ * block_len of block table[t / block_len]; a block outside [0, num_blocks)
+ * reads as rows of zeros.  Lengths are clamped to what the tables hold.
+ *   out = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m)),
+ *   s_j = softmax_scale * (q . k_j); a row that sees nothing is zeros.
+ * Scores, sums and the accumulation are fp32; the probabilities enter the
+ * matrix instructions as bf16.  FP8 caches are attended as stored (fold a
+ * scale into softmax_scale and the output).  The cached positions of a prefix
+ * are read once for all rows of a tile (up to 64 query rows of one kv head),
+ * not once per sequence.  Workspace: mkd_shared_prefix_workspace_bytes(args)
+ * (depends on the shapes alone); calls that share it must not overlap. */
+typedef struct {
+  const void* q;
+  long long q_stride[3];       /* sequence, new token, head (elements, multiples of 8) */
+  void* out;                   /* bf16 */
+  long long out_stride[3];
+  const void *k_cache, *v_cache; /* rows start on 16-byte boundaries */
+  long long k_cache_stride[3], v_cache_stride[3];
+  int num_blocks, block_len;
+  int kv_format;
+  const int* prefix_tables;    /* [G, prefix_blocks] */
+  const int* prefix_lens;      /* [G] */
+  const int* prefix_starts;    /* [G + 1] */
+  const int* tables;           /* [B, own_blocks] */
+  const int* lens;             /* [B] */
+  int G, prefix_blocks, own_blocks;
+  float softmax_scale;
+  const float* sink;           /* [nq] or NULL */
+  int B, s_tkg, nq, nkv, d;
+} mkd_shared_prefix_args;
+size_t mkd_shared_prefix_workspace_bytes(const mkd_shared_prefix_args* args);
+int mkd_attention_shared_prefix(const mkd_shared_prefix_args* args, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* mkd_sample_tokens: one token per row of logits [B, V] (bf16 or fp32) from a
+ * given uniform random number in [0, 1).  The tokens of a row in order of
+ * falling logit (ties: the lowest index first), with masses e_j = exp((l_j -
+ * l_0) / temperature):
+ *   top_k > 0: the first top_k;   top_p < 1: of those, every token before
+ *   which less than top_p of their mass lies (the first always);   min_p: of
+ *   those, the ones with e_j >= min_p (the first always);
+ * tokens[b] is the first of them whose cumulative mass exceeds uniforms[b]
+ * times their mass, logprobs[b] (or NULL) the logarithm of its share of it.
+ * temperature <= 0: the first token.  -inf and NaN logits are never chosen; a
+ * +inf logit leaves no mass to finite ones; a row with nothing to choose gives
+ * -1 and -inf.  Masses are formed in fp64 and summed so that the order of the
+ * additions does not matter: equal inputs give equal tokens.  Each setting is
+ * a value for all rows, or [B] in device memory (its pointer not NULL).
+ * 1 <= V <= 2^20. */
+typedef struct {
+  const void* logits;
+  int logits_dtype;            /* MKD_DT_* */
+  long long row_stride;        /* elements */
+  const float* uniforms;       /* [B] */
+  float temperature, top_p, min_p;
+  int top_k;
+  const float *temperature_rows, *top_p_rows, *min_p_rows; /* [B] or NULL */
+  const int* top_k_rows;
+  int* tokens;                 /* [B] */
+  float* logprobs;             /* [B] or NULL */
+  int B, V;
+} mkd_sample_args;
+size_t mkd_sample_workspace_bytes(int B, int V);
+int mkd_sample_tokens(const mkd_sample_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

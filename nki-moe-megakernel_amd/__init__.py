@@ -7,6 +7,10 @@ Operator surface (same names, argument order and defaults as the reference):
   moe_tkg               nki_kernels/moe/moe_tkg.py:56
   moe_prefill           moe_tkg for prefill-shaped batches (T > 128; no
                         reference counterpart), LDS-tiled MFMA GEMMs
+Serving many samples of a few prompts on a paged KV cache (no reference counterparts):
+  kv_append_rope           new tokens' heads normed, rotated and appended
+  attention_shared_prefix  decode attention that reads a shared prefix once
+  sample_tokens            temperature, top-k, top-p, min-p from given random numbers
 Model surface:
   qwen_with_megakernel  megakernels/qwen3_moe/qwen_with_megakernel.py
   gpt_oss_with_megakernel  megakernels/gpt_oss/gpt_oss_with_megakernel.py
@@ -25,6 +29,8 @@ from .common_types import (ActFnType, ExpertAffinityScaleMode, QuantizationType,
                            RouterActFnType)
 from .moe import moe_prefill, moe_tkg, router_topk
 from .norm import rmsnorm_tkg
+from .paged import attention_shared_prefix, kv_append_rope
+from .sample import sample_tokens
 
-__all__ = ["rmsnorm_tkg", "attention_block_tkg", "router_topk", "moe_tkg", "moe_prefill", "ActFnType",
-           "ExpertAffinityScaleMode", "QuantizationType", "RouterActFnType"]
+__all__ = ["rmsnorm_tkg", "attention_block_tkg", "router_topk", "moe_tkg", "moe_prefill", "kv_append_rope",
+           "attention_shared_prefix", "sample_tokens", "ActFnType", "ExpertAffinityScaleMode", "QuantizationType", "RouterActFnType"]

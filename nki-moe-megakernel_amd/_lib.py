@@ -7,6 +7,7 @@ libmkd binds to (both carry the SONAME libamdhip64.so.7).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -91,6 +92,38 @@ KV_FP8 = 1            # MKD_KV_FP8
 KV_K_TRANSPOSED = 2   # MKD_KV_K_TRANSPOSED
 
 
+class KvAppendArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("x_dtype", i32),
+        ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2),
+        ("q_out", vp), ("q_out_stride", i64 * 2), ("q_norm", vp), ("k_norm", vp), ("eps", f32),
+        ("cos", vp), ("sin", vp), ("table_rows", i32), ("rot", i32), ("positions", vp), ("positions_i64", i32),
+        ("k_cache", vp), ("v_cache", vp), ("k_cache_stride", i64 * 3), ("v_cache_stride", i64 * 3),
+        ("num_blocks", i32), ("block_len", i32), ("kv_format", i32), ("k_scale", vp), ("v_scale", vp),
+        ("slots", vp), ("slots_i64", i32), ("T", i32), ("nq", i32), ("nkv", i32), ("d", i32),
+    ]
+
+
+class SharedPrefixArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("q_stride", i64 * 3), ("out", vp), ("out_stride", i64 * 3),
+        ("k_cache", vp), ("v_cache", vp), ("k_cache_stride", i64 * 3), ("v_cache_stride", i64 * 3),
+        ("num_blocks", i32), ("block_len", i32), ("kv_format", i32),
+        ("prefix_tables", vp), ("prefix_lens", vp), ("prefix_starts", vp), ("tables", vp), ("lens", vp),
+        ("G", i32), ("prefix_blocks", i32), ("own_blocks", i32), ("softmax_scale", f32), ("sink", vp),
+        ("B", i32), ("s_tkg", i32), ("nq", i32), ("nkv", i32), ("d", i32),
+    ]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("logits", vp), ("logits_dtype", i32), ("row_stride", i64), ("uniforms", vp),
+        ("temperature", f32), ("top_p", f32), ("min_p", f32), ("top_k", i32),
+        ("temperature_rows", vp), ("top_p_rows", vp), ("min_p_rows", vp), ("top_k_rows", vp),
+        ("tokens", vp), ("logprobs", vp), ("B", i32), ("V", i32),
+    ]
+
+
 class Qwen3Model(C.Structure):
     _fields_ = [
         ("num_layers", i32), ("H", i32), ("nq", i32), ("nkv", i32), ("d", i32), ("E", i32),
@@ -131,6 +164,11 @@ _SIGS = {
     "mkd_attention_workspace_bytes_tkg": (sz, [i32, i32, i32, i32, i32, i32, i32]),
     "mkd_attention_block_tkg": (i32, [C.POINTER(AttentionArgs), vp, sz, vp]),
     "mkd_attention_prepare_operands": (i32, [C.POINTER(AttentionOperands), vp]),
+    "mkd_kv_append_rope": (i32, [C.POINTER(KvAppendArgs), vp]),
+    "mkd_shared_prefix_workspace_bytes": (sz, [C.POINTER(SharedPrefixArgs)]),
+    "mkd_attention_shared_prefix": (i32, [C.POINTER(SharedPrefixArgs), vp, sz, vp]),
+    "mkd_sample_workspace_bytes": (sz, [i32, i32]),
+    "mkd_sample_tokens": (i32, [C.POINTER(SampleArgs), vp, sz, vp]),
     "mkd_packed_fp8_bytes": (sz, [i32, i32, i32]),
     "mkd_pack_fp8_weights": (i32, [vp, vp, i32, i32, i32, vp]),
     "mkd_qwen3_workspace_bytes": (sz, [C.POINTER(Qwen3Model), i32]),
@@ -204,3 +242,10 @@ def require_gpu(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError("mkd operators take device (HIP) tensors; got a CPU tensor")
+
+
+def on_device(dev):
+    """Context that makes `dev` the current device (nothing to do where it is)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)

@@ -1927,4 +1927,130 @@ int mkd_qwen3_layer_kernel_status(const mkd_qwen3_model* m, int B, const void* w
   return MKD_OK;
 }
 
+// ---- serving many samples of a few prompts ----
+static int check_paged(const char* what, const void* k, const void* v, const long long* ks, const long long* vs,
+                       int num_blocks, int block_len, int nkv, int kv_format, int row_bytes) {
+  const int eb = (kv_format & MKD_KV_FP8) ? 1 : 2;
+  MKD_REQUIRE(kv_format == 0 || kv_format == MKD_KV_FP8, MKD_ERR_UNSUPPORTED, "%s: kv_format %d", what, kv_format);
+  MKD_REQUIRE(num_blocks > 0 && block_len > 0 && nkv > 0 && (long long)num_blocks * block_len < (1LL << 31),
+              MKD_ERR_INVALID, "%s: pool of %d blocks of %d rows, %d heads", what, num_blocks, block_len, nkv);
+  for (int i = 0; i < 3; ++i)
+    MKD_REQUIRE(ks[i] >= 0 && vs[i] >= 0 && ks[i] * eb % row_bytes == 0 && vs[i] * eb % row_bytes == 0,
+                MKD_ERR_INVALID, "%s: cache strides must be non-negative multiples of %d bytes", what, row_bytes);
+  MKD_REQUIRE(reinterpret_cast<uintptr_t>(k) % row_bytes == 0 && reinterpret_cast<uintptr_t>(v) % row_bytes == 0,
+              MKD_ERR_INVALID, "%s: caches must start on multiples of %d bytes", what, row_bytes);
+  return MKD_OK;
+}
+
+int mkd_kv_append_rope(const mkd_kv_append_args* a, void* stream) {
+  if (int rc = stale_check("mkd_kv_append_rope")) return rc;
+  MKD_REQUIRE(a, MKD_ERR_NULL, "kv_append_rope: null pointer");
+  MKD_REQUIRE(a->T >= 0 && a->nq > 0 && a->nkv > 0 && (long long)a->T * (a->nq + 2LL * a->nkv) < (1LL << 31),
+              MKD_ERR_INVALID, "kv_append_rope: %d tokens of %d + 2 x %d heads", a->T, a->nq, a->nkv);
+  MKD_REQUIRE(a->d == 64 || a->d == 128, MKD_ERR_UNSUPPORTED, "kv_append_rope: d %d (64 or 128)", a->d);
+  MKD_REQUIRE(a->x_dtype == MKD_DT_F32 || a->x_dtype == MKD_DT_BF16, MKD_ERR_INVALID, "kv_append_rope: x_dtype %d",
+              a->x_dtype);
+  MKD_REQUIRE(!a->cos == !a->sin, MKD_ERR_NULL, "kv_append_rope: cos and sin go together");
+  MKD_REQUIRE(a->cos ? (a->rot > 0 && a->rot <= a->d && a->rot % 8 == 0 && a->table_rows > 0) : a->rot == 0,
+              MKD_ERR_INVALID, "kv_append_rope: rot %d of d %d, %d table rows", a->rot, a->d, a->table_rows);
+  if (int rc = check_paged("kv_append_rope", a->k_cache, a->v_cache, a->k_cache_stride, a->v_cache_stride, a->num_blocks,
+                           a->block_len, a->nkv, a->kv_format, a->kv_format ? 4 : 8))
+    return rc;
+  if (a->T == 0) return MKD_OK;
+  MKD_REQUIRE(a->q && a->k && a->v && a->q_out && a->k_cache && a->v_cache && a->slots, MKD_ERR_NULL,
+              "kv_append_rope: null pointer");
+  MKD_REQUIRE(!a->cos || a->positions, MKD_ERR_NULL, "kv_append_rope: rotation needs positions");
+  MKD_REQUIRE(!(a->kv_format & MKD_KV_FP8) || (a->k_scale && a->v_scale), MKD_ERR_NULL,
+              "kv_append_rope: an FP8 cache needs k_scale and v_scale");
+  const uintptr_t in = a->x_dtype == MKD_DT_F32 ? 15 : 7;
+  const uintptr_t xs = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v);
+  const uintptr_t tabs = reinterpret_cast<uintptr_t>(a->cos) | reinterpret_cast<uintptr_t>(a->sin);
+  const uintptr_t bfs = reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->q_norm) |
+                        reinterpret_cast<uintptr_t>(a->k_norm);
+  bool quads = (xs & in) == 0 && (tabs & 15) == 0 && (bfs & 7) == 0;
+  for (int i = 0; i < 2; ++i)
+    quads = quads && a->q_stride[i] % 4 == 0 && a->k_stride[i] % 4 == 0 && a->v_stride[i] % 4 == 0 && a->q_out_stride[i] % 4 == 0;
+  MKD_REQUIRE(quads, MKD_ERR_INVALID, "kv_append_rope: rows must start on multiples of 4 elements");
+  MKD_TRY(kv_append_launch(*a, static_cast<hipStream_t>(stream)), "kv_append_rope");
+  return MKD_OK;
+}
+
+static int check_shared(const mkd_shared_prefix_args* a) {
+  MKD_REQUIRE(a, MKD_ERR_NULL, "attention_shared_prefix: null pointer");
+  MKD_REQUIRE(a->d == 64 || a->d == 128, MKD_ERR_UNSUPPORTED, "attention_shared_prefix: d %d (64 or 128)", a->d);
+  MKD_REQUIRE(a->B >= 0 && a->B <= 65535 && a->s_tkg >= 1 && a->s_tkg <= 8, MKD_ERR_INVALID,
+              "attention_shared_prefix: B %d (to 65535), s_tkg %d (1 to 8)", a->B, a->s_tkg);
+  MKD_REQUIRE(a->nq > 0 && a->nkv > 0 && a->nq % a->nkv == 0 && a->nq <= 4096, MKD_ERR_INVALID,
+              "attention_shared_prefix: %d query heads over %d kv heads", a->nq, a->nkv);
+  MKD_REQUIRE(a->G >= 0 && a->G <= 65535 && a->prefix_blocks >= 0 && a->own_blocks >= 0 && a->block_len > 0 &&
+                  (long long)a->prefix_blocks * a->block_len < (1LL << 30) && (long long)a->own_blocks * a->block_len < (1LL << 30),
+              MKD_ERR_INVALID, "attention_shared_prefix: %d groups of %d blocks, %d own blocks of %d rows", a->G,
+              a->prefix_blocks, a->own_blocks, a->block_len);
+  const SharedPlan p = shared_plan(*a);
+  MKD_REQUIRE((a->B == 0 || p.prefix_tiles <= 65535) && p.prefix_chunks * a->nkv < (1LL << 30) &&
+                  p.own_chunks * a->nkv < (1LL << 30) && (long long)a->B * a->s_tkg * a->nq < (1LL << 31),
+              MKD_ERR_UNSUPPORTED, "attention_shared_prefix: too many row tiles (%lld) or positions for one call", p.prefix_tiles);
+  return MKD_OK;
+}
+
+size_t mkd_shared_prefix_workspace_bytes(const mkd_shared_prefix_args* a) {
+  if (check_shared(a)) return 0;
+  const SharedPlan p = shared_plan(*a);
+  const size_t parts = (size_t)a->B * a->s_tkg * a->nq * (p.prefix_chunks + p.own_chunks);
+  Carver c{nullptr, 0};
+  c.take<float>(parts * a->d);
+  c.take<float>(parts * 2);
+  return c.used;
+}
+
+int mkd_attention_shared_prefix(const mkd_shared_prefix_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = stale_check("mkd_attention_shared_prefix")) return rc;
+  if (int rc = check_shared(a)) return rc;
+  if (int rc = check_paged("attention_shared_prefix", a->k_cache, a->v_cache, a->k_cache_stride, a->v_cache_stride,
+                           a->num_blocks, a->block_len, a->nkv, a->kv_format, 16))
+    return rc;
+  if (a->B == 0) return MKD_OK;
+  const SharedPlan p = shared_plan(*a);
+  MKD_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->lens && (a->tables || a->own_blocks == 0) &&
+                  (a->G == 0 || (a->prefix_lens && a->prefix_starts && (a->prefix_tables || a->prefix_blocks == 0))),
+              MKD_ERR_NULL, "attention_shared_prefix: null pointer");
+  bool rows = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && reinterpret_cast<uintptr_t>(a->out) % 4 == 0;
+  for (int i = 0; i < 3; ++i) rows = rows && a->q_stride[i] % 8 == 0 && a->out_stride[i] % 2 == 0;
+  MKD_REQUIRE(rows, MKD_ERR_INVALID, "attention_shared_prefix: query rows must start on multiples of 8 elements, output rows of 2");
+  SharedArgs s{};
+  s.p = *a;
+  s.prefix_chunk = p.prefix_chunk;
+  s.own_chunk = p.own_chunk;
+  s.prefix_chunks = (int)p.prefix_chunks;
+  s.slots = (int)(p.prefix_chunks + p.own_chunks);
+  const size_t parts = (size_t)a->B * a->s_tkg * a->nq * s.slots;
+  Carver c{static_cast<char*>(workspace), workspace_bytes};
+  s.part_o = c.take<float>(parts * a->d);
+  s.part_ml = c.take<float>(parts * 2);
+  MKD_REQUIRE(c.ok && (workspace || c.used == 0), MKD_ERR_WORKSPACE, "attention_shared_prefix: workspace %zu < %zu bytes",
+              workspace_bytes, c.used);
+  MKD_TRY(attn_shared_launch(s, p, static_cast<hipStream_t>(stream)), "attention_shared_prefix");
+  return MKD_OK;
+}
+
+size_t mkd_sample_workspace_bytes(int B, int V) {
+  return B > 0 && V > 0 && V <= (1 << 20) ? sample_workspace(B, V) : 0;
+}
+
+int mkd_sample_tokens(const mkd_sample_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = stale_check("mkd_sample_tokens")) return rc;
+  MKD_REQUIRE(a, MKD_ERR_NULL, "sample_tokens: null pointer");
+  MKD_REQUIRE(a->B >= 0 && a->B <= 65535 && a->V >= 1 && a->V <= (1 << 20), MKD_ERR_INVALID,
+              "sample_tokens: %d rows (to 65535) of %d logits (1 to 2^20)", a->B, a->V);
+  MKD_REQUIRE(a->logits_dtype == MKD_DT_F32 || a->logits_dtype == MKD_DT_BF16, MKD_ERR_INVALID,
+              "sample_tokens: logits_dtype %d", a->logits_dtype);
+  MKD_REQUIRE(a->row_stride >= 0, MKD_ERR_INVALID, "sample_tokens: row_stride %lld", a->row_stride);
+  if (a->B == 0) return MKD_OK;
+  MKD_REQUIRE(a->logits && a->uniforms && a->tokens && workspace, MKD_ERR_NULL, "sample_tokens: null pointer");
+  MKD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= sample_workspace(a->B, a->V),
+              MKD_ERR_WORKSPACE, "sample_tokens: workspace %zu < %zu bytes", workspace_bytes, sample_workspace(a->B, a->V));
+  MKD_TRY(sample_launch(*a, workspace, static_cast<hipStream_t>(stream)), "sample_tokens");
+  return MKD_OK;
+}
+
 }  // extern "C"

@@ -562,6 +562,25 @@ hipError_t moe_finalize_launch(const float* ybuf, int T, int K, int H, const int
                                const uint16_t* resid, uint16_t* out, float* out_f32, hipStream_t s);
 
 // misc.hip
+// kv_append.hip
+hipError_t kv_append_launch(const mkd_kv_append_args& a, hipStream_t s);
+// attn_shared.hip: how a call's positions split into blocks, from its shapes alone
+struct SharedPlan {
+  int prefix_qt, own_qt, own_tiles;       // 16-row tiles per block; tiles of one sequence's rows
+  long long prefix_tiles;                 // row tiles of all groups, at most
+  int prefix_chunk, own_chunk;            // positions per block
+  long long prefix_chunks, own_chunks;
+};
+struct SharedArgs {
+  mkd_shared_prefix_args p;
+  int prefix_chunk, own_chunk, prefix_chunks, slots;   // slots: partials per row
+  float *part_o, *part_ml;                // [rows][slots][d], [rows][slots][2]
+};
+SharedPlan shared_plan(const mkd_shared_prefix_args& p);
+hipError_t attn_shared_launch(const SharedArgs& a, const SharedPlan& p, hipStream_t s);
+// sample.hip
+size_t sample_workspace(int B, int V);
+hipError_t sample_launch(const mkd_sample_args& a, void* ws, hipStream_t s);
 hipError_t attn_operands_launch(const mkd_attention_operands& o, hipStream_t s);
 hipError_t embed_launch(const int* ids, const uint16_t* table, uint16_t* out, int B, int H, int V,
                         hipStream_t s);
