@@ -7,7 +7,6 @@ libmkd binds to (both carry the SONAME libamdhip64.so.7).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 
@@ -92,13 +91,18 @@ KV_FP8 = 1            # MKD_KV_FP8
 KV_K_TRANSPOSED = 2   # MKD_KV_K_TRANSPOSED
 
 
+def _steps(name, n):
+    """The n strides of an array field, one field each (filled faster from Python)."""
+    return [(f"{name}{i}", i64) for i in range(n)]
+
+
 class KvAppendArgs(C.Structure):
     _fields_ = [
         ("q", vp), ("k", vp), ("v", vp), ("x_dtype", i32),
-        ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2),
-        ("q_out", vp), ("q_out_stride", i64 * 2), ("q_norm", vp), ("k_norm", vp), ("eps", f32),
+        *_steps("q_stride", 2), *_steps("k_stride", 2), *_steps("v_stride", 2),
+        ("q_out", vp), *_steps("q_out_stride", 2), ("q_norm", vp), ("k_norm", vp), ("eps", f32),
         ("cos", vp), ("sin", vp), ("table_rows", i32), ("rot", i32), ("positions", vp), ("positions_i64", i32),
-        ("k_cache", vp), ("v_cache", vp), ("k_cache_stride", i64 * 3), ("v_cache_stride", i64 * 3),
+        ("k_cache", vp), ("v_cache", vp), *_steps("k_cache_stride", 3), *_steps("v_cache_stride", 3),
         ("num_blocks", i32), ("block_len", i32), ("kv_format", i32), ("k_scale", vp), ("v_scale", vp),
         ("slots", vp), ("slots_i64", i32), ("T", i32), ("nq", i32), ("nkv", i32), ("d", i32),
     ]
@@ -106,8 +110,8 @@ class KvAppendArgs(C.Structure):
 
 class SharedPrefixArgs(C.Structure):
     _fields_ = [
-        ("q", vp), ("q_stride", i64 * 3), ("out", vp), ("out_stride", i64 * 3),
-        ("k_cache", vp), ("v_cache", vp), ("k_cache_stride", i64 * 3), ("v_cache_stride", i64 * 3),
+        ("q", vp), *_steps("q_stride", 3), ("out", vp), *_steps("out_stride", 3),
+        ("k_cache", vp), ("v_cache", vp), *_steps("k_cache_stride", 3), *_steps("v_cache_stride", 3),
         ("num_blocks", i32), ("block_len", i32), ("kv_format", i32),
         ("prefix_tables", vp), ("prefix_lens", vp), ("prefix_starts", vp), ("tables", vp), ("lens", vp),
         ("G", i32), ("prefix_blocks", i32), ("own_blocks", i32), ("softmax_scale", f32), ("sink", vp),
@@ -244,8 +248,27 @@ def require_gpu(*tensors):
             raise ValueError("mkd operators take device (HIP) tensors; got a CPU tensor")
 
 
-def on_device(dev):
-    """Context that makes `dev` the current device (nothing to do where it is)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def gpu_index(**tensors) -> int:
+    """The GPU that all the given tensors are on (None: absent)."""
+    dev = None
+    for name, t in tensors.items():
+        if t is not None:
+            at = t.get_device()
+            if at != dev:
+                if at < 0:
+                    raise ValueError(f"mkd operators take device (HIP) tensors; {name} is a CPU tensor")
+                if dev is not None:
+                    raise ValueError(f"{name} is on GPU {at}, the tensors before it on GPU {dev}")
+                dev = at
+    return dev
+
+
+def call(fn, what: str, index: int, *args):
+    """fn(*args, stream) on the current stream of GPU `index`, errors raised."""
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != MKD_OK:
+        check(rc, what)

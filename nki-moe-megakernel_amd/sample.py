@@ -46,24 +46,23 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Set
     never chosen; a row with nothing to choose gives -1 and -inf.  The result does not depend on the
     order of any addition: equal inputs give equal tokens.  `output`: an int32 [B] tensor for the tokens.
     """
-    L.require_gpu(logits, uniforms, output)
+    index = L.gpu_index(logits=logits, uniforms=uniforms, output=output)
     dev = logits.device
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"logits must be bfloat16 or float32 [B, V], got {logits.dtype} {tuple(logits.shape)}")
     B, V = logits.shape
     if not 1 <= V <= 1 << 20:
         raise ValueError(f"V must be in [1, 2^20], got {V}")
-    if uniforms.dtype != torch.float32 or uniforms.dim() != 1 or uniforms.numel() != B or uniforms.device != dev:
-        raise ValueError(f"uniforms must be float32 [B={B}] on {dev}, got {uniforms.dtype} {tuple(uniforms.shape)} "
-                         f"on {uniforms.device}")
+    if uniforms.dtype != torch.float32 or uniforms.dim() != 1 or uniforms.numel() != B:
+        raise ValueError(f"uniforms must be float32 [B={B}], got {uniforms.dtype} {tuple(uniforms.shape)}")
     t, t_rows = _setting(temperature, "temperature", B, dev, 0.0, 3.4e38)
     k, k_rows = _setting(top_k, "top_k", B, dev, 0, math.inf)
     p, p_rows = _setting(top_p, "top_p", B, dev, 0.0, 1.0)
     m, m_rows = _setting(min_p, "min_p", B, dev, 0.0, 1.0)
     if output is None:
         output = torch.empty(B, dtype=torch.int32, device=dev)
-    elif output.dtype != torch.int32 or tuple(output.shape) != (B,) or output.device != dev or not output.is_contiguous():
-        raise ValueError(f"output must be a contiguous int32 [{B}] tensor on {dev}")
+    elif output.dtype != torch.int32 or tuple(output.shape) != (B,) or not output.is_contiguous():
+        raise ValueError(f"output must be a contiguous int32 [{B}] tensor")
     logprobs = torch.empty(B, dtype=torch.float32, device=dev)
     if B == 0:
         return output, logprobs
@@ -75,7 +74,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Set
         uniforms.data_ptr(), t, p, m, k, L.ptr(t_rows), L.ptr(p_rows), L.ptr(m_rows), L.ptr(k_rows),
         output.data_ptr(), logprobs.data_ptr(), B, V)
     lib = L.load()
-    with L.on_device(dev):
-        ws = torch.empty(lib.mkd_sample_workspace_bytes(B, V), dtype=torch.uint8, device=dev)
-        L.check(lib.mkd_sample_tokens(args, ws.data_ptr(), ws.numel(), L.stream_ptr(dev)), "sample_tokens")
+    n = lib.mkd_sample_workspace_bytes(B, V)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    L.call(lib.mkd_sample_tokens, "sample_tokens", index, args, ws.data_ptr(), n)
     return output, logprobs
