@@ -4,21 +4,22 @@
 // With the tokens in falling order of logit, every filter keeps a front part and the
 // random number asks for the first token whose cumulative mass passes a target: each is
 // a weighted selection, "the first token at which a count or a mass reaches T".
-//   1. chunks: block (4096 logits, row): masses exp((l - chunk max) / temperature) into
-//      512 bins of 1/16 of scaled logit, at fixed places of that scale (so the chunks'
-//      bins line up whatever their maxima), the members of each bin listed.
-//   2. rows: one block joins the chunks' bins, scans them, and finds each filter's end
-//      and then the token: the bin by its cumulative count or mass, then the exact logit
-//      inside the bin by histograms over its members' bit patterns (ordered like the
-//      logits, 10 bits a time), then among equal logits the index by rank.
+//   1. chunks: block (4096 logits, row): the tokens counted and weighed in 512 bins of
+//      1/16 of logit / temperature, at fixed places of that scale (so the chunks' bins
+//      line up whatever their maxima), and listed by bin.
+//   2. rows: one block adds the chunks' bins, scans them, and finds each filter's end and
+//      then the token.  Where the tokens that can stay are few (1024 at most: the usual
+//      top-k, a peaked top-p), they are sorted once and every question is a lookup.
+//      Otherwise the bin is found by its cumulative count or mass, and the token in the
+//      bin by a histogram over its members' bit patterns and a sort of what is left.
 // Tokens 512 bins (32, e^-32) below the maximum get no mass: together at most 2^-26 of
 // the row's for 2^20 of them.
 //
 // The answer is a whole number, and a sum off in its last places would change it where a
-// border lies near: masses are formed in fp64 and summed as 64-bit integers (of 2^-50 of
-// the chunk's largest, 2^-42 of the bin's), which no order of atomic additions changes;
-// only the joining of chunks is in fp64, in a fixed order.  Bound by reading the logits
-// for large batches and by the two dependent launches for small ones.
+// border lies near.  A token's weight is therefore exp(z - middle of its bin), z = logit /
+// temperature in fp64, as an integer of 37 bits (the bin's unit, exp(middle - z_max), joins
+// in fp64 per bin): sums of a bin are exact, whatever the order of atomic additions, and
+// its relative precision does not depend on how far below the maximum it lies.
 #include "common.h"
 #include "mkd_internal.h"
 
@@ -26,16 +27,19 @@ namespace mkd {
 
 namespace {
 
+typedef unsigned long long u64;
 constexpr int kSmChunk = 4096, kSmThreads = 256, kSmPer = kSmChunk / kSmThreads;
 constexpr int kSmBins = 512;
-constexpr double kSmRes = 16.0;                 // bins per unit of logit / temperature
+constexpr double kSmRes = 16.0;                 // bins per unit of z
 constexpr int kSmMaxChunks = (1 << 20) / kSmChunk;
-constexpr int kSmRow = 1024;                    // threads of a row's block, sub-bins of a level
+constexpr int kSmRow = 1024;                    // threads of a row's block, sub-bins, tokens sorted
 constexpr int kSmStage = 8192;                  // members of a bin held in LDS
+constexpr int kSmMassBits = 50;                 // a chunk's bin: count above, mass (4096 weights) below
+constexpr double kSmOne = 0x1p37;               // weight of the middle of a bin; at its edges 3 % off
 
 // What stage 1 leaves per (row, chunk).
 struct SmRecord {
-  unsigned long long mass[kSmBins];             // of 2^-50
+  u64 bins[kSmBins];                            // count << kSmMassBits | mass
   uint16_t list[kSmChunk];                      // positions in the chunk, by bin
   uint16_t start[kSmBins + 8];                  // of bin j in `list`; [kSmBins]: their number
   float top;                                    // the chunk's largest logit
@@ -56,6 +60,7 @@ MKD_DEV SmSetting setting_of(const mkd_sample_args& a, int b) {
   s.min_p = a.min_p_rows ? a.min_p_rows[b] : a.min_p;
   s.u = a.uniforms[b];
   if (!(s.u > 0.0)) s.u = 0.0;
+  if (s.u >= 1.0) s.u = 1.0 - 0x1p-24;
   return s;
 }
 // exp((l - top) * inv_t), 1 for l = top whatever it is, 0 below an infinite top
@@ -64,13 +69,20 @@ MKD_DEV double mass_of(float l, float top, double inv_t) {
   if (top == INFINITY) return 0.0;
   return exp(((double)l - (double)top) * inv_t);
 }
-// the bin's place on the scale of logit / temperature (monotone in l)
+// the bin's place on the scale of z (monotone in l)
 MKD_DEV double place_of(float l, double inv_t) { return floor((double)l * inv_t * kSmRes); }
-// bins between a logit and a larger one (kSmBins: outside)
-MKD_DEV int bins_below(float l, float top, double inv_t) {
-  if (l == top) return 0;
-  const double d = place_of(top, inv_t) - place_of(l, inv_t);
-  return d < kSmBins ? (int)d : kSmBins;        // (an infinite difference: outside)
+// A token's weight from its place: the distance y from the bin's middle is within 1/32,
+// so six terms of the exponential series leave 2^-47; + 2^52 rounds to a whole number.
+MKD_DEV u64 weight_of(float l, double place, double inv_t) {
+  const double y = fma(place, -1.0 / kSmRes, (double)l * inv_t) - 0.5 / kSmRes;
+  double p = 1.0 / 720;
+  p = fma(p, y, 1.0 / 120);
+  p = fma(p, y, 1.0 / 24);
+  p = fma(p, y, 1.0 / 6);
+  p = fma(p, y, 0.5);
+  p = fma(p, y, 1.0);
+  p = fma(p, y, 1.0);
+  return __double_as_longlong(fma(p, kSmOne, 0x1p52)) & ((1ull << 52) - 1);
 }
 // bit patterns in the order of the logits; -0 and +0 are one value
 MKD_DEV uint32_t key_of(float l) {
@@ -78,6 +90,9 @@ MKD_DEV uint32_t key_of(float l) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 MKD_DEV float logit_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+// a token in the falling order, as one number that rises: ~key above, index below
+MKD_DEV u64 token_of(uint32_t key, uint32_t index) { return (u64)~key << 32 | index; }
+MKD_DEV uint32_t key_in(u64 token) { return ~(uint32_t)(token >> 32); }
 
 template <bool BF>
 MKD_DEV float logit_at(const mkd_sample_args& a, long long row, int i) {
@@ -92,15 +107,15 @@ MKD_DEV float logit_at(const mkd_sample_args& a, long long row, int i) {
 // (bf16: 8 x + 2048 (i / 8) + i % 8).
 template <bool BF, bool VEC>
 __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_args a, SmRecord* rec) {
-  __shared__ unsigned long long mass[kSmBins];
-  __shared__ unsigned count[kSmBins];
+  __shared__ u64 bins[kSmBins];
+  __shared__ unsigned first[kSmBins];
   __shared__ __attribute__((aligned(16))) uint16_t list[kSmChunk];
   __shared__ float wtop[kSmThreads / 64];
   __shared__ unsigned wsum[kSmThreads / 64];
   const int x = threadIdx.x, lane = x & 63, w = x >> 6;
   const int b = blockIdx.y, base = blockIdx.x * kSmChunk, n = min(kSmChunk, a.V - base);
   SmRecord& r = rec[(long long)b * gridDim.x + blockIdx.x];
-  for (int i = x; i < kSmBins; i += kSmThreads) { mass[i] = 0; count[i] = 0; }
+  for (int i = x; i < kSmBins; i += kSmThreads) bins[i] = 0;
   const SmSetting s = setting_of(a, b);
   constexpr int G = BF ? 8 : 4;                 // elements of a 16-byte piece
   float l[kSmPer];
@@ -128,20 +143,23 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
   top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
   if (x == 0) r.top = top;
   if (top == -INFINITY) return;                 // nothing to choose here (the rest is not read)
-  uint16_t bin[kSmPer], rank[kSmPer];
+  const double top_place = place_of(top, s.inv_t);
+  uint32_t at[kSmPer];                          // bin << 16 | place among its members
 #pragma unroll
   for (int i = 0; i < kSmPer; ++i) {
-    bin[i] = kSmBins;
-    if (l[i] == -INFINITY) continue;
-    const int j = bins_below(l[i], top, s.inv_t);
-    if (j >= kSmBins) continue;
-    bin[i] = (uint16_t)j;
-    rank[i] = (uint16_t)atomicAdd(&count[j], 1u);
-    atomicAdd(&mass[j], (unsigned long long)rint(mass_of(l[i], top, s.inv_t) * 0x1p50));
+    at[i] = kSmBins << 16;
+    const double place = place_of(l[i], s.inv_t), below = top_place - place;
+    // (below an infinite maximum everything is outside; -inf always is)
+    const bool same = l[i] == top;
+    if (!(same || below < kSmBins) || l[i] == -INFINITY) continue;
+    const int j = same ? 0 : (int)below;
+    const u64 add = (1ull << kSmMassBits) | (top == INFINITY ? (u64)kSmOne : weight_of(l[i], place, s.inv_t));
+    at[i] = j << 16 | (uint32_t)(atomicAdd(&bins[j], add) >> kSmMassBits);
   }
   __syncthreads();
   // exclusive scan of the counts, two bins a thread
-  const unsigned c0 = count[2 * x], c1 = count[2 * x + 1];
+  const u64 b0 = bins[2 * x], b1 = bins[2 * x + 1];
+  const unsigned c0 = (unsigned)(b0 >> kSmMassBits), c1 = (unsigned)(b1 >> kSmMassBits);
   unsigned sum = c0 + c1;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -156,53 +174,45 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
     if (q < w) before += wsum[q];
     total += wsum[q];
   }
-  count[2 * x] = before;
-  count[2 * x + 1] = before + c0;
+  first[2 * x] = before;
+  first[2 * x + 1] = before + c0;
   reinterpret_cast<uint32_t*>(r.start)[x] = before | ((before + c0) << 16);
   if (x == 0) r.start[kSmBins] = (uint16_t)total;
-  r.mass[2 * x] = mass[2 * x];
-  r.mass[2 * x + 1] = mass[2 * x + 1];
+  r.bins[2 * x] = b0;
+  r.bins[2 * x + 1] = b1;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSmPer; ++i)
-    if (bin[i] < kSmBins) list[count[bin[i]] + rank[i]] = (uint16_t)(G * x + G * kSmThreads * (i / G) + i % G);
+    if (at[i] >> 16 < kSmBins)
+      list[first[at[i] >> 16] + (at[i] & 0xffff)] = (uint16_t)(G * x + G * kSmThreads * (i / G) + i % G);
   __syncthreads();
   for (unsigned i = x * 8; i < total; i += kSmThreads * 8) st16(r.list + i, ld16(list + i));
 }
 
 namespace {
 
-// A place in the falling order: the `ties`-th lowest index (from 1) among the members of
-// `bin` with bit pattern `key`; `mass`: of everything up to it.
-struct SmCut {
-  int bin;
-  uint32_t key, ties;
-  double mass;
-};
-MKD_DEV bool later(const SmCut& a, const SmCut& b) {
-  if (a.bin != b.bin) return a.bin > b.bin;
-  return a.key != b.key ? a.key < b.key : a.ties > b.ties;
-}
-
 struct SmShared {
-  double factor[kSmMaxChunks];                  // chunk's mass unit in the row's
-  double cum[kSmBins];                          // mass up to bin j, itself included
-  unsigned long long sub_mass[kSmRow], wave_m[kSmRow / 64];
+  double cum[kSmBins];                          // mass up to bin j, itself included, of the maximum's
+  double unit[kSmBins];                         // mass of weight 1 in bin j
+  u64 bins[kSmBins];                            // weight in bin j
+  u64 sub[kSmRow];                              // sub-bins' weights; the sort's exchange; sorted tokens' masses
+  u64 token[kSmRow];                            // a few tokens
+  u64 wave_m[kSmRow / 64];
+  double wave_d[kSmRow / 64];
+  u64 found_m;
   unsigned cum_n[kSmBins];
   unsigned sub_n[kSmRow], wave_n[kSmRow / 64];
-  double wave_d[kSmRow / 64];
   int shift[kSmMaxChunks];                      // chunk's first bin in the row's
-  unsigned first[kSmMaxChunks + 1];             // the staged bin's members before chunk c
+  unsigned first[kSmMaxChunks + 1];             // the staged members before chunk c
   unsigned at[kSmMaxChunks];                    // where they start in the chunk's list
   uint32_t key[kSmStage], index[kSmStage];
   unsigned hits[kSmMaxChunks], bits[kSmChunk / 32];
-  unsigned long long found_m;
   unsigned found_n;
-  int found, token;
+  int found;
   uint32_t kmin, kmax;
 };
 
-// Inclusive scan over the block's 1024 threads (a thread's own total last).
+// Inclusive scans over the block's 1024 threads.
 MKD_DEV void scan_n(SmShared& s, unsigned& v) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -215,32 +225,67 @@ MKD_DEV void scan_n(SmShared& s, unsigned& v) {
   for (int q = 0; q < w; ++q) v += s.wave_n[q];
   __syncthreads();
 }
-MKD_DEV void scan_m(SmShared& s, unsigned long long& v) {
+template <typename T>
+MKD_DEV void scan_nm(SmShared& s, T* wave, unsigned& n, T& m) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long up = __shfl_up(v, o, 64);
-    if (lane >= o) v += up;
+    const unsigned un = __shfl_up(n, o, 64);
+    const T um = __shfl_up(m, o, 64);
+    if (lane >= o) {
+      n += un;
+      m += um;
+    }
   }
-  if (lane == 63) s.wave_m[w] = v;
+  if (lane == 63) {
+    s.wave_n[w] = n;
+    wave[w] = m;
+  }
   __syncthreads();
-  for (int q = 0; q < w; ++q) v += s.wave_m[q];
+  T front = 0;
+  for (int q = 0; q < w; ++q) {
+    n += s.wave_n[q];
+    front += wave[q];
+  }
+  m += front;
   __syncthreads();
 }
-MKD_DEV void scan_d(SmShared& s, double& v) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// How many threads say so.
+MKD_DEV unsigned count_of(SmShared& s, bool yes) {
+  const unsigned c = (unsigned)__popcll(__ballot(yes));
+  if ((threadIdx.x & 63) == 0) s.wave_n[threadIdx.x >> 6] = c;
+  __syncthreads();
+  unsigned v = 0;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(v, o, 64);
-    if (lane >= o) v += up;
-  }
-  if (lane == 63) s.wave_d[w] = v;
+  for (int q = 0; q < kSmRow / 64; ++q) v += s.wave_n[q];
   __syncthreads();
-  double before = 0.0;
-  for (int q = 0; q < w; ++q) before += s.wave_d[q];
-  v += before;
-  __syncthreads();
+  return v;
 }
+// Rising bitonic sort of one number per thread among the first `n` threads (the others
+// hold ~0): strides inside a wave by shuffles, longer ones through LDS.
+MKD_DEV u64 sort_up(SmShared& s, u64 v, unsigned n) {
+  const unsigned x = threadIdx.x;
+  for (unsigned size = 2; size / 2 < n; size <<= 1)
+    for (unsigned stride = size >> 1; stride > 0; stride >>= 1) {
+      u64 o;
+      if (stride < 64) {
+        o = __shfl_xor(v, (int)stride, 64);
+      } else {
+        s.sub[x] = v;
+        __syncthreads();
+        o = s.sub[x ^ stride];
+        __syncthreads();
+      }
+      const bool keep_low = ((x & stride) == 0) == ((x & size) == 0);
+      v = (v < o) == keep_low ? v : o;
+    }
+  return v;
+}
+
+struct SmEnd {
+  u64 token;                                    // the last one kept (or a number behind it)
+  double mass;                                  // of everything up to it
+};
 
 template <bool BF>
 struct SmRow {
@@ -253,6 +298,11 @@ struct SmRow {
   int staged = -1;
   unsigned n = 0;                               // members of the staged bin
 
+  MKD_DEV u64 weight(uint32_t key) const {
+    if (top == INFINITY) return (u64)kSmOne;
+    const float l = logit_of(key);
+    return weight_of(l, place_of(l, inv_t), inv_t);
+  }
   // member m of the staged bin: its index, and its logit's bit pattern
   MKD_DEV void member(unsigned m, uint32_t& key, uint32_t& index) const {
     if (n <= kSmStage) {
@@ -272,16 +322,14 @@ struct SmRow {
     index = lo * kSmChunk + rec[lo].list[s.at[lo] + m - s.first[lo]];
     key = key_of(logit_at<BF>(a, b, index));
   }
-  MKD_DEV void stage(int bin) {
-    if (staged == bin) return;
-    staged = bin;
+  // the members of bins [from, bin]: their number in each chunk, and where they are listed
+  MKD_DEV unsigned locate(int from, int bin) {
     __syncthreads();
     const int c = threadIdx.x;
     unsigned cnt = 0, at = 0;
-    if (c < nc && rec[c].top != -INFINITY && s.shift[c] <= bin && bin - s.shift[c] < kSmBins) {
-      const int j = bin - s.shift[c];
-      at = rec[c].start[j];
-      cnt = rec[c].start[j + 1] - at;
+    if (c < nc && s.shift[c] <= bin) {          // (a chunk without tokens lies behind every bin)
+      at = rec[c].start[max(from - s.shift[c], 0)];
+      cnt = rec[c].start[bin - s.shift[c] + 1] - at;
     }
     unsigned v = cnt;
     scan_n(s, v);
@@ -290,9 +338,15 @@ struct SmRow {
       s.at[c] = at;
       if (c == nc - 1) s.first[nc] = v;
     }
-    if (c == 0) { s.kmin = 0xffffffffu; s.kmax = 0u; }
     __syncthreads();
-    n = s.first[nc];
+    return s.first[nc];
+  }
+  MKD_DEV void stage(int bin) {
+    if (staged == bin) return;
+    staged = bin;
+    n = locate(bin, bin);
+    if (threadIdx.x == 0) { s.kmin = 0xffffffffu; s.kmax = 0u; }
+    __syncthreads();
     uint32_t lo = 0xffffffffu, hi = 0u;
     for (unsigned m = threadIdx.x; m < n; m += kSmRow) {
       uint32_t key, index;
@@ -310,26 +364,19 @@ struct SmRow {
     }
     __syncthreads();
   }
-  // a member's mass, of 2^-42 of the bin's largest
-  MKD_DEV unsigned long long weight(uint32_t key, float bin_top) const {
-    return (unsigned long long)rint(mass_of(logit_of(key), bin_top, inv_t) * 0x1p42);
-  }
-  // The first member (by falling logit, equal ones by index) of `bin` at which the count
-  // (by_count) or the integer mass reaches want >= 1; the last one if none does.
-  MKD_DEV SmCut select(int bin, bool by_count, unsigned long long want, double mass_before) {
+  // The first member (in falling order) of `bin` at which the count (by_count) or the
+  // weight reaches want >= 1, the last one if none does.
+  MKD_DEV SmEnd select(int bin, bool by_count, u64 want) {
     stage(bin);
     const uint32_t kmax = s.kmax;
-    const float bin_top = logit_of(kmax);
-    const double unit = mass_of(bin_top, top, inv_t);
-    uint32_t base = 0, range = kmax - s.kmin;   // distances kmax - key in [base, base + range]
-    unsigned long long before = 0;              // mass in front of them
+    uint32_t base = 0, range = kmax - s.kmin;   // members' distances kmax - key: [base, base + range]
+    unsigned left = n;                          // members there
+    u64 front = 0;                              // weight before them
     const int x = threadIdx.x;
-    uint32_t at_key;
-    unsigned at_n;
-    for (;;) {
-      const int bits = range ? 32 - __clz(range) : 0, shift = bits > 10 ? bits - 10 : 0;
+    while (left > kSmRow && range > 0) {
+      const int bits = 32 - __clz(range), shift = bits > 10 ? bits - 10 : 0;
       s.sub_n[x] = 0;
-      s.sub_mass[x] = 0;
+      s.sub[x] = 0;
       if (x == 0) s.found = -1;
       __syncthreads();
       for (unsigned m = x; m < n; m += kSmRow) {
@@ -338,18 +385,16 @@ struct SmRow {
         const uint32_t d = kmax - key;
         if (d < base || d - base > range) continue;
         atomicAdd(&s.sub_n[(d - base) >> shift], 1u);
-        atomicAdd(&s.sub_mass[(d - base) >> shift], weight(key, bin_top));
+        atomicAdd(&s.sub[(d - base) >> shift], weight(key));
       }
       __syncthreads();
       const unsigned cn = s.sub_n[x];
-      const unsigned long long cm = s.sub_mass[x];
+      const u64 cm = s.sub[x];
       unsigned sn = cn;
-      unsigned long long sm = cm;
-      scan_n(s, sn);
-      scan_m(s, sm);
-      const unsigned long long upto = by_count ? sn : sm;
+      u64 sm = cm;
+      scan_nm(s, s.wave_m, sn, sm);
       // the sub-bin that reaches it, or the last one with members
-      if (cn && upto >= want && (by_count ? sn - cn : sm - cm) < want) s.found = x;
+      if (cn && (by_count ? sn : sm) >= want && (by_count ? sn - cn : sm - cm) < want) s.found = x;
       __syncthreads();
       const bool none = s.found < 0;
       __syncthreads();
@@ -363,66 +408,82 @@ struct SmRow {
         s.found_m = sm - cm;
       }
       __syncthreads();
-      const unsigned long long front = by_count ? s.found_n : s.found_m;
-      want = want > front ? want - front : 1;
-      before += s.found_m;
+      const u64 passed = by_count ? s.found_n : s.found_m;
+      want = want > passed ? want - passed : 1;
+      front += s.found_m;
       base += (uint32_t)hit << shift;
-      at_n = s.sub_n[hit];
-      __syncthreads();
-      if (shift == 0) {
-        at_key = kmax - base;
-        break;
-      }
+      left = s.sub_n[hit];
       range = (1u << shift) - 1u;
+      __syncthreads();
     }
-    const unsigned long long each = by_count ? 1ull : max(weight(at_key, bin_top), 1ull);
-    const unsigned long long ties = min((want + each - 1) / each, (unsigned long long)at_n);
-    SmCut c;
-    c.bin = bin;
-    c.key = at_key;
-    c.ties = (uint32_t)max(ties, 1ull);
-    c.mass = mass_before + (double)(before + c.ties * weight(at_key, bin_top)) * 0x1p-42 * unit;
-    return c;
+    if (left > kSmRow) return equal_ones(bin, kmax - base, by_count, want, front, left);
+    // ---- what is left, sorted ----
+    if (x == 0) s.found_n = 0;
+    __syncthreads();
+    for (unsigned m = x; m < n; m += kSmRow) {
+      uint32_t key, index;
+      member(m, key, index);
+      const uint32_t d = kmax - key;
+      if (d >= base && d - base <= range) s.token[atomicAdd(&s.found_n, 1u)] = token_of(key, index);
+    }
+    __syncthreads();
+    const u64 t = sort_up(s, x < (int)left ? s.token[x] : ~0ull, left);
+    unsigned c = x < (int)left ? 1u : 0u;
+    const u64 own = c ? weight(key_in(t)) : 0ull;
+    u64 m = own;
+    scan_nm(s, s.wave_m, c, m);
+    const unsigned pos = count_of(s, x + 1 < (int)left && (by_count ? c : m) < want);
+    if (x == (int)pos) {
+      s.token[0] = t;
+      s.found_m = m;
+    }
+    __syncthreads();
+    const SmEnd e{s.token[0], before(bin) + (double)(front + s.found_m) * s.unit[bin]};
+    __syncthreads();
+    return e;
   }
-  // the index that a cut names
-  MKD_DEV int index_of(const SmCut& c) {
-    stage(c.bin);
+  // more equal members than are sorted: the one at which it reaches `want`, by index
+  MKD_DEV SmEnd equal_ones(int bin, uint32_t key, bool by_count, u64 want, u64 front, unsigned left) {
+    const u64 each = weight(key);
+    const unsigned rank = (unsigned)min(by_count ? want : (want + each - 1) / each, (u64)left);   // from 1
     const int x = threadIdx.x;
     if (x < nc) s.hits[x] = 0;
     if (x < kSmChunk / 32) s.bits[x] = 0;
     __syncthreads();
     for (unsigned m = x; m < n; m += kSmRow) {
-      uint32_t key, index;
-      member(m, key, index);
-      if (key == c.key) atomicAdd(&s.hits[index / kSmChunk], 1u);
+      uint32_t k, index;
+      member(m, k, index);
+      if (k == key) atomicAdd(&s.hits[index / kSmChunk], 1u);
     }
     __syncthreads();
     unsigned v = x < nc ? s.hits[x] : 0, own = v;
     scan_n(s, v);
-    if (x < nc && v >= c.ties && v - own < c.ties) {
+    if (x < nc && v >= rank && v - own < rank) {
       s.found = x;
-      s.found_n = c.ties - (v - own);           // its rank in that chunk, from 1
+      s.found_n = rank - (v - own);             // its rank in that chunk, from 1
     }
     __syncthreads();
     const int chunk = s.found;
-    const unsigned rank = s.found_n;
+    const unsigned in_chunk = s.found_n;
     for (unsigned m = x; m < n; m += kSmRow) {
-      uint32_t key, index;
-      member(m, key, index);
-      if (key == c.key && (int)(index / kSmChunk) == chunk)
-        atomicOr(&s.bits[index % kSmChunk / 32], 1u << (index % 32));
+      uint32_t k, index;
+      member(m, k, index);
+      if (k == key && (int)(index / kSmChunk) == chunk) atomicOr(&s.bits[index % kSmChunk / 32], 1u << (index % 32));
     }
     __syncthreads();
     uint32_t word = x < kSmChunk / 32 ? s.bits[x] : 0;
     v = own = __popc(word);
     scan_n(s, v);
-    if (v >= rank && v - own < rank) {
-      for (unsigned k = rank - (v - own); k > 1; --k) word &= word - 1;
-      s.token = chunk * kSmChunk + 32 * x + __ffs((int)word) - 1;
+    if (v >= in_chunk && v - own < in_chunk) {
+      for (unsigned k = in_chunk - (v - own); k > 1; --k) word &= word - 1;
+      s.token[0] = token_of(key, chunk * kSmChunk + 32 * x + __ffs((int)word) - 1);
     }
     __syncthreads();
-    return s.token;
+    const SmEnd e{s.token[0], before(bin) + (double)(front + rank * each) * s.unit[bin]};
+    __syncthreads();
+    return e;
   }
+  MKD_DEV double before(int bin) const { return bin > 0 ? s.cum[bin - 1] : 0.0; }
 };
 
 }  // namespace
@@ -433,13 +494,12 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
   const int b = blockIdx.x, x = threadIdx.x;
   rec += (long long)b * nc;
   const SmSetting set = setting_of(a, b);
-  // ---- the row's largest logit, each chunk's place and unit ----
+  // ---- the row's largest logit, and each chunk's place below it ----
   const float mine = x < nc ? rec[x].top : -INFINITY;
   float top = wave_max(mine);                   // (chunks are 256 at most: the first 4 waves)
   if ((x & 63) == 0) s.wave_d[x >> 6] = top;
   __syncthreads();
-  top = -INFINITY;
-  for (int q = 0; q < kSmRow / 64; ++q) top = fmaxf(top, (float)s.wave_d[q]);
+  top = (float)fmax(fmax(s.wave_d[0], s.wave_d[1]), fmax(s.wave_d[2], s.wave_d[3]));
   if (top == -INFINITY) {                       // nothing to choose
     if (x == 0) {
       a.tokens[b] = -1;
@@ -447,33 +507,38 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     }
     return;
   }
+  const double top_place = place_of(top, set.inv_t);
   if (x < nc) {
-    const bool live = mine != -INFINITY;
-    s.shift[x] = live ? bins_below(mine, top, set.inv_t) : kSmBins;
-    s.factor[x] = live ? mass_of(mine, top, set.inv_t) * 0x1p-50 : 0.0;
+    const double d = mine == top ? 0.0 : top_place - place_of(mine, set.inv_t);
+    s.shift[x] = d < kSmBins ? (int)d : kSmBins;
   }
   __syncthreads();
   // ---- the row's bins: two threads each, even and odd chunks ----
   {
     const int j = x >> 1;
     unsigned cnt = 0;
-    double m = 0.0;
+    u64 m = 0;
+#pragma unroll 8
     for (int c = x & 1; c < nc; c += 2) {
       const int k = j - s.shift[c];
-      if (k < 0) continue;                      // (a chunk without tokens: its shift is past every bin)
-      cnt += rec[c].start[k + 1] - rec[c].start[k];
-      m += (double)rec[c].mass[k] * s.factor[c];
+      const u64 v = rec[c].bins[max(k, 0)];     // (what a chunk without tokens holds is not used)
+      if (k >= 0) {
+        cnt += (unsigned)(v >> kSmMassBits);
+        m += v & ((1ull << kSmMassBits) - 1);
+      }
     }
     cnt += __shfl_xor(cnt, 1, 64);
-    const double other = __shfl_xor(m, 1, 64);
-    m = (x & 1) ? other + m : m + other;
+    m += __shfl_xor(m, 1, 64);
+    // exp(middle - z_max): both from the maximum's place, so that no large number is subtracted
+    const double unit = top == INFINITY ? 1.0 / kSmOne
+        : exp(fma(top_place, 1.0 / kSmRes, -((double)top * set.inv_t)) + (0.5 - j) / kSmRes) / kSmOne;
     unsigned sn = (x & 1) ? 0 : cnt;
-    double sm = (x & 1) ? 0.0 : m;
-    scan_n(s, sn);
-    scan_d(s, sm);
+    double sm = (x & 1) ? 0.0 : (double)m * unit;
+    scan_nm(s, s.wave_d, sn, sm);
     if (!(x & 1)) {
       s.cum_n[j] = sn;
       s.cum[j] = sm;
+      s.unit[j] = unit;
     }
   }
   __syncthreads();
@@ -481,7 +546,6 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
   // the first bin that reaches a target; `last` if none does
   int last = kSmBins - 1;
   auto find_bin = [&](auto reached) {
-    __syncthreads();
     if (x == 0) s.found = last;
     __syncthreads();
     if (x < kSmBins && reached(x)) atomicMin(&s.found, x);
@@ -490,28 +554,69 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     __syncthreads();
     return j;
   };
-  auto before = [&](int j) { return j > 0 ? s.cum[j - 1] : 0.0; };
-  auto members = [&](int j) { return s.cum_n[j] - (j > 0 ? s.cum_n[j - 1] : 0u); };
-  // integer mass of a bin's front part that holds t of the row's units
-  auto in_bin = [&](int j, double t, bool past) -> unsigned long long {
-    row.stage(j);
-    const double v = t / mass_of(logit_of(s.kmax), top, set.inv_t) * 0x1p42;
-    if (!(v > 0.0)) return 1;
-    return v < 0x1p63 ? (past ? (unsigned long long)v + 1 : (unsigned long long)ceil(v)) : ~0ull >> 1;
-  };
-  last = find_bin([&](int i) { return s.cum_n[i] >= s.cum_n[kSmBins - 1]; });   // the last with members
+  const unsigned tokens = s.cum_n[kSmBins - 1];
   const double all = s.cum[kSmBins - 1];
-  SmCut end{kSmBins, 0u, 0u, all};              // behind everything
-  if (set.top_k > 0 && (unsigned)set.top_k < s.cum_n[kSmBins - 1]) {
-    const unsigned k = set.top_k;
-    const int j = find_bin([&](int i) { return s.cum_n[i] >= k; });
-    end = row.select(j, true, k - (j > 0 ? s.cum_n[j - 1] : 0u), before(j));
+  last = find_bin([&](int i) { return s.cum_n[i] >= tokens; });   // the last with members
+  const bool by_k = set.top_k > 0 && (unsigned)set.top_k < tokens, by_p = set.top_p < 1.0;
+  const int jk = by_k ? find_bin([&](int i) { return s.cum_n[i] >= (unsigned)set.top_k; }) : last;
+  // ---- few tokens can stay: sort them ----
+  // (all of the first top_k, whose mass top_p refers to; else those that top_p or min_p,
+  // or without a filter the random number, can reach at most)
+  int far = jk;
+  if (!by_k) {
+    far = last;
+    if (set.min_p > 0.0 && top != INFINITY)     // one bin to spare
+      far = (int)fmin(floor(((double)top * set.inv_t - log(set.min_p)) * kSmRes - top_place) + 1.0, (double)last);
+    if (by_p || !(set.min_p > 0.0)) {
+      const double most = (by_p ? set.top_p : set.u) * all;
+      const int j = find_bin([&](int i) { return by_p ? s.cum[i] >= most : s.cum[i] > most; });
+      far = min(far, j);
+    }
   }
-  if (set.top_p < 1.0) {
+  far = max(far, 0);
+  if (s.cum_n[far] <= kSmRow) {
+    const unsigned n = row.locate(0, far);
+    u64 t = ~0ull;
+    if (x < (int)n) {
+      uint32_t key, index;
+      row.fetch(x, key, index);
+      t = token_of(key, index);
+    }
+    t = sort_up(s, t, n);
+    const float l = logit_of(key_in(t));
+    const double own = x < (int)n ? mass_of(l, top, set.inv_t) : 0.0;
+    unsigned c = 0;
+    double cum = own;
+    scan_nm(s, s.wave_d, c, cum);
+    double* at = reinterpret_cast<double*>(s.sub);
+    at[x] = cum;
+    __syncthreads();
+    unsigned kept = by_k ? min((unsigned)set.top_k, n) : n;
+    const double whole = n == tokens ? at[n - 1] : all;   // (sorted: without the bins' rounding)
+    const double m1 = by_k ? at[kept - 1] : whole;
+    if (by_p) kept = max(min(kept, count_of(s, x < (int)kept && cum - own < set.top_p * m1)), 1u);
+    if (set.min_p > 0.0) kept = max(count_of(s, x < (int)kept && own >= set.min_p), 1u);
+    // (without a filter the whole row's mass counts; the tokens sorted reach past u of it)
+    const double m3 = by_k || by_p || set.min_p > 0.0 ? at[kept - 1] : whole;
+    const unsigned pick = min(count_of(s, x < (int)kept && cum <= set.u * m3), kept - 1);
+    if (x == (int)pick) {
+      a.tokens[b] = (int)(uint32_t)t;
+      if (a.logprobs) a.logprobs[b] = (float)log(own / m3);
+    }
+    return;
+  }
+  // integer weight of a bin's front part that holds t of the row's mass
+  auto in_bin = [&](int j, double t, bool past) -> u64 {
+    const double v = (t - row.before(j)) / s.unit[j];
+    if (!(v > 0.0)) return 1;
+    return v < 0x1p62 ? (past ? (u64)v + 1 : (u64)ceil(v)) : 1ull << 62;
+  };
+  SmEnd end{~0ull, all};                        // behind everything
+  if (by_k) end = row.select(jk, true, set.top_k - (jk > 0 ? s.cum_n[jk - 1] : 0u));
+  if (by_p) {
     const double t = set.top_p * end.mass;
-    const int j = find_bin([&](int i) { return s.cum[i] >= t && members(i); });
-    const SmCut c = row.select(j, false, in_bin(j, t - before(j), false), before(j));
-    if (later(end, c)) end = c;
+    const int j = find_bin([&](int i) { return s.cum[i] >= t; });
+    end = row.select(j, false, in_bin(j, t, false));
   }
   if (set.min_p > 0.0) {
     // the smallest logit whose mass is min_p at least, from its estimate by steps of one
@@ -524,42 +629,32 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
       for (int i = 0; i < 64 && mass_of(logit_of(k - 1), top, set.inv_t) >= set.min_p; ++i) --k;
       cut = logit_of(k);
     }
-    const int j = bins_below(cut, top, set.inv_t);
-    if (j < end.bin || (j == end.bin && key_of(cut) > end.key)) {
-      // the members of bin j at least as large: a selection by their number
-      row.stage(min(j, kSmBins - 1));
-      if (x == 0) s.found_n = 0;
-      __syncthreads();
-      unsigned hits = 0;
-      if (j < kSmBins)
-        for (unsigned m = x; m < row.n; m += kSmRow) {
-          uint32_t key, index;
-          row.member(m, key, index);
-          hits += key >= key_of(cut);
-        }
-      if (hits) atomicAdd(&s.found_n, hits);
-      __syncthreads();
-      hits = s.found_n;
-      __syncthreads();
-      if (hits) {
-        end = row.select(j, true, hits, before(j));
-      } else if (j < kSmBins) {                 // everything in front of the bin
-        const double m = before(j);
-        const int i = find_bin([&](int q) { return s.cum_n[q] >= (j > 0 ? s.cum_n[j - 1] : 0u); });
-        end = SmCut{i, 0u, 0xffffffffu, m};     // (a place behind the bin's last member)
+    const uint32_t key = key_of(cut);
+    const double below = cut == top ? 0.0 : top_place - place_of(cut, set.inv_t);
+    if (token_of(key, 0xffffffffu) < end.token && below < kSmBins) {
+      const int j = (int)below;
+      row.stage(j);                             // the weight of the bin's members at least as large
+      u64 m = 0;
+      for (unsigned i = x; i < row.n; i += kSmRow) {
+        uint32_t k, index;
+        row.member(i, k, index);
+        if (k >= key) m += row.weight(k);
       }
+      unsigned c = 0;
+      scan_nm(s, s.wave_m, c, m);
+      if (x == kSmRow - 1) s.found_m = m;
+      __syncthreads();
+      end = SmEnd{token_of(key, 0xffffffffu), row.before(j) + (double)s.found_m * s.unit[j]};
+      __syncthreads();
     }
   }
   // ---- the token: the first whose cumulative mass passes u times the kept ----
   const double t = set.u * end.mass;
-  int j = find_bin([&](int i) { return s.cum[i] > t && members(i); });
-  if (j > end.bin) j = end.bin;
-  SmCut pick = row.select(j, false, in_bin(j, t - before(j), true), before(j));
-  if (later(pick, end)) pick = end;
-  const int token = row.index_of(pick);
+  const int j = find_bin([&](int i) { return s.cum[i] > t; });
+  const SmEnd pick = row.select(j, false, in_bin(j, t, true));
   if (x == 0) {
-    a.tokens[b] = token;
-    if (a.logprobs) a.logprobs[b] = (float)log(mass_of(logit_of(pick.key), top, set.inv_t) / end.mass);
+    a.tokens[b] = (int)(uint32_t)pick.token;
+    if (a.logprobs) a.logprobs[b] = (float)log(mass_of(logit_of(key_in(pick.token)), top, set.inv_t) / end.mass);
   }
 }
 
