@@ -4,20 +4,20 @@
 // With the tokens in falling order of logit, every filter keeps a front part and the
 // random number asks for the first token whose cumulative mass passes a target: each is
 // a weighted selection, "the first token at which a count or a mass reaches T".
-//   1. chunks: block (4096 logits, row): the tokens counted and weighed in 512 bins of
+//   1. chunks: block (8192 logits, row): the tokens counted and weighed in 512 bins of
 //      1/16 of logit / temperature, at fixed places of that scale (so the chunks' bins
 //      line up whatever their maxima), and listed by bin.
 //   2. rows: one block adds the chunks' bins, scans them, and finds each filter's end and
-//      then the token.  Where the tokens that can stay are few (1024 at most: the usual
+//      then the token.  Where the tokens that can stay are few (512 at most: the usual
 //      top-k, a peaked top-p), they are sorted once and every question is a lookup.
 //      Otherwise the bin is found by its cumulative count or mass, and the token in the
-//      bin by a histogram over its members' bit patterns and a sort of what is left.
+//      bin by histograms over its members' bit patterns until a wave can sort the rest.
 // Tokens 512 bins (32, e^-32) below the maximum get no mass: together at most 2^-26 of
 // the row's for 2^20 of them.
 //
 // The answer is a whole number, and a sum off in its last places would change it where a
 // border lies near.  A token's weight is therefore exp(z - middle of its bin), z = logit /
-// temperature in fp64, as an integer of 37 bits (the bin's unit, exp(middle - z_max), joins
+// temperature in fp64, as an integer of 36 bits (the bin's unit, exp(middle - z_max), joins
 // in fp64 per bin): sums of a bin are exact, whatever the order of atomic additions, and
 // its relative precision does not depend on how far below the maximum it lies.
 #include "common.h"
@@ -28,14 +28,14 @@ namespace mkd {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kSmChunk = 4096, kSmThreads = 256, kSmPer = kSmChunk / kSmThreads;
+constexpr int kSmChunk = 8192, kSmThreads = 512, kSmPer = kSmChunk / kSmThreads;
 constexpr int kSmBins = 512;
 constexpr double kSmRes = 16.0;                 // bins per unit of z
 constexpr int kSmMaxChunks = (1 << 20) / kSmChunk;
-constexpr int kSmRow = 1024;                    // threads of a row's block, sub-bins, tokens sorted
+constexpr int kSmRow = 512;                     // threads of a row's block: a bin each
 constexpr int kSmStage = 8192;                  // members of a bin held in LDS
 constexpr int kSmMassBits = 50;                 // a chunk's bin: count above, mass (4096 weights) below
-constexpr double kSmOne = 0x1p37;               // weight of the middle of a bin; at its edges 3 % off
+constexpr double kSmOne = 0x1p36;               // weight of the middle of a bin; at its edges 3 % off
 
 // What stage 1 leaves per (row, chunk).
 struct SmRecord {
@@ -84,12 +84,17 @@ MKD_DEV u64 weight_of(float l, double place, double inv_t) {
   p = fma(p, y, 1.0);
   return __double_as_longlong(fma(p, kSmOne, 0x1p52)) & ((1ull << 52) - 1);
 }
-// bit patterns in the order of the logits; -0 and +0 are one value
+// bit patterns in the order of the logits (a bf16 one's upper half); -0 and +0 are one value
+template <bool BF>
 MKD_DEV uint32_t key_of(float l) {
   const uint32_t u = __float_as_uint(l + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (u & 0x80000000u ? ~u : u | 0x80000000u) >> (BF ? 16 : 0);
 }
-MKD_DEV float logit_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+template <bool BF>
+MKD_DEV float logit_of(uint32_t k) {
+  if constexpr (BF) return __uint_as_float((k & 0x8000u ? k & 0x7fffu : ~k) << 16);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
 // a token in the falling order, as one number that rises: ~key above, index below
 MKD_DEV u64 token_of(uint32_t key, uint32_t index) { return (u64)~key << 32 | index; }
 MKD_DEV uint32_t key_in(u64 token) { return ~(uint32_t)(token >> 32); }
@@ -103,8 +108,8 @@ MKD_DEV float logit_at(const mkd_sample_args& a, long long row, int i) {
 
 }  // namespace
 
-// VEC: rows on 16-byte boundaries.  Element i of thread x is 4 x + 1024 (i / 4) + i % 4
-// (bf16: 8 x + 2048 (i / 8) + i % 8).
+// VEC: rows on 16-byte boundaries.  Element i of thread x is 4 x + 2048 (i / 4) + i % 4
+// (bf16: 8 x + 4096 (i / 8) + i % 8).
 template <bool BF, bool VEC>
 __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_args a, SmRecord* rec) {
   __shared__ u64 bins[kSmBins];
@@ -140,7 +145,8 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
   top = wave_max(top);
   if (lane == 0) wtop[w] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
+#pragma unroll
+  for (int q = 0; q < kSmThreads / 64; ++q) top = fmaxf(top, wtop[q]);
   if (x == 0) r.top = top;
   if (top == -INFINITY) return;                 // nothing to choose here (the rest is not read)
   const double top_place = place_of(top, s.inv_t);
@@ -157,10 +163,11 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
     at[i] = j << 16 | (uint32_t)(atomicAdd(&bins[j], add) >> kSmMassBits);
   }
   __syncthreads();
-  // exclusive scan of the counts, two bins a thread
-  const u64 b0 = bins[2 * x], b1 = bins[2 * x + 1];
-  const unsigned c0 = (unsigned)(b0 >> kSmMassBits), c1 = (unsigned)(b1 >> kSmMassBits);
-  unsigned sum = c0 + c1;
+  // exclusive scan of the counts, a bin a thread
+  static_assert(kSmBins == kSmThreads, "one bin a thread");
+  const u64 mine = bins[x];
+  const unsigned cnt = (unsigned)(mine >> kSmMassBits);
+  unsigned sum = cnt;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const unsigned up = __shfl_up(sum, o, 64);
@@ -168,18 +175,16 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
   }
   if (lane == 63) wsum[w] = sum;
   __syncthreads();
-  unsigned before = sum - c0 - c1, total = 0;
+  unsigned before = sum - cnt, total = 0;
 #pragma unroll
   for (int q = 0; q < kSmThreads / 64; ++q) {
     if (q < w) before += wsum[q];
     total += wsum[q];
   }
-  first[2 * x] = before;
-  first[2 * x + 1] = before + c0;
-  reinterpret_cast<uint32_t*>(r.start)[x] = before | ((before + c0) << 16);
+  first[x] = before;
+  r.start[x] = (uint16_t)before;
   if (x == 0) r.start[kSmBins] = (uint16_t)total;
-  r.bins[2 * x] = b0;
-  r.bins[2 * x + 1] = b1;
+  r.bins[x] = mine;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSmPer; ++i)
@@ -196,7 +201,7 @@ struct SmShared {
   double unit[kSmBins];                         // mass of weight 1 in bin j
   u64 bins[kSmBins];                            // weight in bin j
   u64 sub[kSmRow];                              // sub-bins' weights; the sort's exchange; sorted tokens' masses
-  u64 token[kSmRow];                            // a few tokens
+  u64 token[64], found_t;                       // a few tokens, and one
   u64 wave_m[kSmRow / 64];
   double wave_d[kSmRow / 64];
   u64 found_m;
@@ -209,10 +214,12 @@ struct SmShared {
   unsigned hits[kSmMaxChunks], bits[kSmChunk / 32];
   unsigned found_n;
   int found;
-  uint32_t kmin, kmax;
+  uint32_t wave_lo[kSmRow / 64], wave_hi[kSmRow / 64];
 };
 
-// Inclusive scans over the block's 1024 threads.
+static_assert(kSmRow == kSmBins && kSmChunk / 32 <= kSmRow && kSmMaxChunks <= kSmRow, "one of each per thread");
+
+// Inclusive scans over the block's threads.
 MKD_DEV void scan_n(SmShared& s, unsigned& v) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -297,10 +304,11 @@ struct SmRow {
   double inv_t;
   int staged = -1;
   unsigned n = 0;                               // members of the staged bin
+  uint32_t kmin = 0, kmax = 0;                  // their least and largest bit patterns
 
   MKD_DEV u64 weight(uint32_t key) const {
     if (top == INFINITY) return (u64)kSmOne;
-    const float l = logit_of(key);
+    const float l = logit_of<BF>(key);
     return weight_of(l, place_of(l, inv_t), inv_t);
   }
   // member m of the staged bin: its index, and its logit's bit pattern
@@ -309,18 +317,38 @@ struct SmRow {
       key = s.key[m];
       index = s.index[m];
     } else {
-      fetch(m, key, index);
+      uint32_t k[1], i[1];
+      fetch<1>(m, k, i);
+      key = k[0];
+      index = i[0];
     }
   }
-  MKD_DEV void fetch(unsigned m, uint32_t& key, uint32_t& index) const {
-    int lo = 0, hi = nc;                        // the chunk: first[lo] <= m < first[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s.first[mid] <= m) lo = mid;
-      else hi = mid;
+  // members m, m + kSmRow, .. (N of them; those behind the last repeat it): their chunks by
+  // bisection (first[lo] <= m), the loads of all in flight together
+  template <int N>
+  MKD_DEV void fetch(unsigned m, uint32_t (&key)[N], uint32_t (&index)[N]) const {
+    unsigned at[N];
+    int lo[N];
+    const unsigned end = s.first[nc] - 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      at[i] = min(m + i * kSmRow, end);
+      lo[i] = 0;
     }
-    index = lo * kSmChunk + rec[lo].list[s.at[lo] + m - s.first[lo]];
-    key = key_of(logit_at<BF>(a, b, index));
+#pragma unroll
+    for (int step = kSmMaxChunks / 2; step > 0; step >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int to = lo[i] + step;
+        if (to < nc && s.first[to] <= at[i]) lo[i] = to;
+      }
+#pragma unroll
+    for (int i = 0; i < N; ++i) index[i] = rec[lo[i]].list[s.at[lo[i]] + at[i] - s.first[lo[i]]];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      index[i] += lo[i] * kSmChunk;
+      key[i] = key_of<BF>(logit_at<BF>(a, b, index[i]));
+    }
   }
   // the members of bins [from, bin]: their number in each chunk, and where they are listed
   MKD_DEV unsigned locate(int from, int bin) {
@@ -345,51 +373,83 @@ struct SmRow {
     if (staged == bin) return;
     staged = bin;
     n = locate(bin, bin);
-    if (threadIdx.x == 0) { s.kmin = 0xffffffffu; s.kmax = 0u; }
-    __syncthreads();
     uint32_t lo = 0xffffffffu, hi = 0u;
-    for (unsigned m = threadIdx.x; m < n; m += kSmRow) {
-      uint32_t key, index;
-      fetch(m, key, index);
-      if (n <= kSmStage) {
-        s.key[m] = key;
-        s.index[m] = index;
+    for (unsigned m = threadIdx.x; m < n; m += 8 * kSmRow) {
+      uint32_t key[8], index[8];
+      fetch<8>(m, key, index);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (n <= kSmStage && m + i * kSmRow < n) {
+          s.key[m + i * kSmRow] = key[i];
+          s.index[m + i * kSmRow] = index[i];
+        }
+        lo = min(lo, key[i]);
+        hi = max(hi, key[i]);
       }
-      lo = min(lo, key);
-      hi = max(hi, key);
     }
-    if (hi >= lo) {
-      atomicMin(&s.kmin, lo);
-      atomicMax(&s.kmax, hi);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
+      hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+      s.wave_lo[threadIdx.x >> 6] = lo;
+      s.wave_hi[threadIdx.x >> 6] = hi;
     }
     __syncthreads();
+    kmin = 0xffffffffu;
+    kmax = 0u;
+#pragma unroll
+    for (int q = 0; q < kSmRow / 64; ++q) {
+      kmin = min(kmin, s.wave_lo[q]);
+      kmax = max(kmax, s.wave_hi[q]);
+    }
   }
   // The first member (in falling order) of `bin` at which the count (by_count) or the
   // weight reaches want >= 1, the last one if none does.
   MKD_DEV SmEnd select(int bin, bool by_count, u64 want) {
     stage(bin);
-    const uint32_t kmax = s.kmax;
-    uint32_t base = 0, range = kmax - s.kmin;   // members' distances kmax - key: [base, base + range]
+    uint32_t base = 0, range = kmax - kmin;   // the members' distances kmax - key: [base, base + range]
     unsigned left = n;                          // members there
     u64 front = 0;                              // weight before them
     const int x = threadIdx.x;
-    while (left > kSmRow && range > 0) {
-      const int bits = 32 - __clz(range), shift = bits > 10 ? bits - 10 : 0;
+    while (left > 64 && range > 0) {
+      const int bits = 32 - __clz(range), shift = bits > 9 ? bits - 9 : 0;
       s.sub_n[x] = 0;
       s.sub[x] = 0;
       if (x == 0) s.found = -1;
       __syncthreads();
-      for (unsigned m = x; m < n; m += kSmRow) {
-        uint32_t key, index;
-        member(m, key, index);
-        const uint32_t d = kmax - key;
-        if (d < base || d - base > range) continue;
-        atomicAdd(&s.sub_n[(d - base) >> shift], 1u);
-        atomicAdd(&s.sub[(d - base) >> shift], weight(key));
+      if (shift == 0) {
+        // one key a sub-bin: counted (few of them, ties among 16-bit logits, by a ballot each:
+        // thousands of atomics on a few words would queue), weighed once
+        for (unsigned m0 = 0; m0 < n; m0 += kSmRow) {
+          uint32_t key = 0, index, d = ~0u;
+          if (m0 + x < n) {
+            member(m0 + x, key, index);
+            d = kmax - key - base;
+          }
+          if (range < 32) {
+            for (uint32_t v = 0; v <= range; ++v) {
+              const u64 same = __ballot(d == v);
+              if (same && (x & 63) == 0) atomicAdd(&s.sub_n[v], (unsigned)__popcll(same));
+            }
+          } else if (d <= range) {
+            atomicAdd(&s.sub_n[d], 1u);
+          }
+        }
+      } else {
+        for (unsigned m = x; m < n; m += kSmRow) {
+          uint32_t key, index;
+          member(m, key, index);
+          const uint32_t d = kmax - key;
+          if (d < base || d - base > range) continue;
+          atomicAdd(&s.sub_n[(d - base) >> shift], 1u);
+          atomicAdd(&s.sub[(d - base) >> shift], weight(key));
+        }
       }
       __syncthreads();
       const unsigned cn = s.sub_n[x];
-      const u64 cm = s.sub[x];
+      const u64 cm = shift == 0 ? (cn ? cn * weight(kmax - (base + x)) : 0ull) : s.sub[x];
       unsigned sn = cn;
       u64 sm = cm;
       scan_nm(s, s.wave_m, sn, sm);
@@ -416,8 +476,8 @@ struct SmRow {
       range = (1u << shift) - 1u;
       __syncthreads();
     }
-    if (left > kSmRow) return equal_ones(bin, kmax - base, by_count, want, front, left);
-    // ---- what is left, sorted ----
+    if (left > 64) return equal_ones(bin, kmax - base, by_count, want, front, left);
+    // ---- what is left, sorted by one wave ----
     if (x == 0) s.found_n = 0;
     __syncthreads();
     for (unsigned m = x; m < n; m += kSmRow) {
@@ -427,18 +487,23 @@ struct SmRow {
       if (d >= base && d - base <= range) s.token[atomicAdd(&s.found_n, 1u)] = token_of(key, index);
     }
     __syncthreads();
-    const u64 t = sort_up(s, x < (int)left ? s.token[x] : ~0ull, left);
-    unsigned c = x < (int)left ? 1u : 0u;
-    const u64 own = c ? weight(key_in(t)) : 0ull;
-    u64 m = own;
-    scan_nm(s, s.wave_m, c, m);
-    const unsigned pos = count_of(s, x + 1 < (int)left && (by_count ? c : m) < want);
-    if (x == (int)pos) {
-      s.token[0] = t;
-      s.found_m = m;
+    if (x < 64) {
+      const u64 t = sort_up(s, x < (int)left ? s.token[x] : ~0ull, left);
+      const u64 own = x < (int)left ? weight(key_in(t)) : 0ull;
+      u64 m = own;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const u64 up = __shfl_up(m, o, 64);
+        if (x >= o) m += up;
+      }
+      const int pos = __popcll(__ballot(x + 1 < (int)left && (by_count ? (u64)x + 1 : m) < want));
+      if (x == pos) {
+        s.found_t = t;
+        s.found_m = m;
+      }
     }
     __syncthreads();
-    const SmEnd e{s.token[0], before(bin) + (double)(front + s.found_m) * s.unit[bin]};
+    const SmEnd e{s.found_t, before(bin) + (double)(front + s.found_m) * s.unit[bin]};
     __syncthreads();
     return e;
   }
@@ -476,10 +541,10 @@ struct SmRow {
     scan_n(s, v);
     if (v >= in_chunk && v - own < in_chunk) {
       for (unsigned k = in_chunk - (v - own); k > 1; --k) word &= word - 1;
-      s.token[0] = token_of(key, chunk * kSmChunk + 32 * x + __ffs((int)word) - 1);
+      s.found_t = token_of(key, chunk * kSmChunk + 32 * x + __ffs((int)word) - 1);
     }
     __syncthreads();
-    const SmEnd e{s.token[0], before(bin) + (double)(front + rank * each) * s.unit[bin]};
+    const SmEnd e{s.found_t, before(bin) + (double)(front + rank * each) * s.unit[bin]};
     __syncthreads();
     return e;
   }
@@ -496,10 +561,10 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
   const SmSetting set = setting_of(a, b);
   // ---- the row's largest logit, and each chunk's place below it ----
   const float mine = x < nc ? rec[x].top : -INFINITY;
-  float top = wave_max(mine);                   // (chunks are 256 at most: the first 4 waves)
+  float top = wave_max(mine);                   // (chunks are 128 at most: the first 2 waves)
   if ((x & 63) == 0) s.wave_d[x >> 6] = top;
   __syncthreads();
-  top = (float)fmax(fmax(s.wave_d[0], s.wave_d[1]), fmax(s.wave_d[2], s.wave_d[3]));
+  top = (float)fmax(s.wave_d[0], s.wave_d[1]);
   if (top == -INFINITY) {                       // nothing to choose
     if (x == 0) {
       a.tokens[b] = -1;
@@ -513,47 +578,40 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     s.shift[x] = d < kSmBins ? (int)d : kSmBins;
   }
   __syncthreads();
-  // ---- the row's bins: two threads each, even and odd chunks ----
+  // ---- the row's bins, one a thread, the loads of 16 chunks in flight together ----
   {
-    const int j = x >> 1;
-    unsigned cnt = 0;
+    unsigned sn = 0;
     u64 m = 0;
-#pragma unroll 8
-    for (int c = x & 1; c < nc; c += 2) {
-      const int k = j - s.shift[c];
-      const u64 v = rec[c].bins[max(k, 0)];     // (what a chunk without tokens holds is not used)
-      if (k >= 0) {
-        cnt += (unsigned)(v >> kSmMassBits);
-        m += v & ((1ull << kSmMassBits) - 1);
+    for (int c0 = 0; c0 < nc; c0 += 16) {
+      u64 v[16];
+      int k[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = min(c0 + i, nc - 1);
+        k[i] = c0 + i < nc ? x - s.shift[c] : -1;
+        v[i] = rec[c].bins[max(k[i], 0)];       // (what a chunk without tokens holds is not used)
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k[i] >= 0) {
+          sn += (unsigned)(v[i] >> kSmMassBits);
+          m += v[i] & ((1ull << kSmMassBits) - 1);
+        }
     }
-    cnt += __shfl_xor(cnt, 1, 64);
-    m += __shfl_xor(m, 1, 64);
     // exp(middle - z_max): both from the maximum's place, so that no large number is subtracted
     const double unit = top == INFINITY ? 1.0 / kSmOne
-        : exp(fma(top_place, 1.0 / kSmRes, -((double)top * set.inv_t)) + (0.5 - j) / kSmRes) / kSmOne;
-    unsigned sn = (x & 1) ? 0 : cnt;
-    double sm = (x & 1) ? 0.0 : (double)m * unit;
+        : exp(fma(top_place, 1.0 / kSmRes, -((double)top * set.inv_t)) + (0.5 - x) / kSmRes) / kSmOne;
+    double sm = (double)m * unit;
     scan_nm(s, s.wave_d, sn, sm);
-    if (!(x & 1)) {
-      s.cum_n[j] = sn;
-      s.cum[j] = sm;
-      s.unit[j] = unit;
-    }
+    s.cum_n[x] = sn;
+    s.cum[x] = sm;
+    s.unit[x] = unit;
   }
   __syncthreads();
   SmRow<BF> row{a, s, rec, b, nc, top, set.inv_t};
-  // the first bin that reaches a target; `last` if none does
+  // the first bin that reaches a target (all behind it do too); `last` if none does
   int last = kSmBins - 1;
-  auto find_bin = [&](auto reached) {
-    if (x == 0) s.found = last;
-    __syncthreads();
-    if (x < kSmBins && reached(x)) atomicMin(&s.found, x);
-    __syncthreads();
-    const int j = s.found;
-    __syncthreads();
-    return j;
-  };
+  auto find_bin = [&](auto reached) { return min((int)count_of(s, !reached(x)), last); };
   const unsigned tokens = s.cum_n[kSmBins - 1];
   const double all = s.cum[kSmBins - 1];
   last = find_bin([&](int i) { return s.cum_n[i] >= tokens; });   // the last with members
@@ -578,12 +636,12 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     const unsigned n = row.locate(0, far);
     u64 t = ~0ull;
     if (x < (int)n) {
-      uint32_t key, index;
-      row.fetch(x, key, index);
-      t = token_of(key, index);
+      uint32_t key[1], index[1];
+      row.template fetch<1>(x, key, index);
+      t = token_of(key[0], index[0]);
     }
     t = sort_up(s, t, n);
-    const float l = logit_of(key_in(t));
+    const float l = logit_of<BF>(key_in(t));
     const double own = x < (int)n ? mass_of(l, top, set.inv_t) : 0.0;
     unsigned c = 0;
     double cum = own;
@@ -605,6 +663,7 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     }
     return;
   }
+  // ---- many: in steps ----
   // integer weight of a bin's front part that holds t of the row's mass
   auto in_bin = [&](int j, double t, bool past) -> u64 {
     const double v = (t - row.before(j)) / s.unit[j];
@@ -624,12 +683,12 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     if (set.min_p < 1.0 && top != INFINITY) {
       cut = fminf((float)((double)top + log(set.min_p) / set.inv_t), top);
       if (cut == -INFINITY) cut = -3.402823466e38f;
-      uint32_t k = key_of(cut);
-      for (int i = 0; i < 64 && logit_of(k) < top && mass_of(logit_of(k), top, set.inv_t) < set.min_p; ++i) ++k;
-      for (int i = 0; i < 64 && mass_of(logit_of(k - 1), top, set.inv_t) >= set.min_p; ++i) --k;
-      cut = logit_of(k);
+      uint32_t k = key_of<BF>(cut);
+      for (int i = 0; i < 64 && logit_of<BF>(k) < top && mass_of(logit_of<BF>(k), top, set.inv_t) < set.min_p; ++i) ++k;
+      for (int i = 0; i < 64 && mass_of(logit_of<BF>(k - 1), top, set.inv_t) >= set.min_p; ++i) --k;
+      cut = logit_of<BF>(k);
     }
-    const uint32_t key = key_of(cut);
+    const uint32_t key = key_of<BF>(cut);
     const double below = cut == top ? 0.0 : top_place - place_of(cut, set.inv_t);
     if (token_of(key, 0xffffffffu) < end.token && below < kSmBins) {
       const int j = (int)below;
@@ -654,7 +713,7 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
   const SmEnd pick = row.select(j, false, in_bin(j, t, true));
   if (x == 0) {
     a.tokens[b] = (int)(uint32_t)pick.token;
-    if (a.logprobs) a.logprobs[b] = (float)log(mass_of(logit_of(key_in(pick.token)), top, set.inv_t) / end.mass);
+    if (a.logprobs) a.logprobs[b] = (float)log(mass_of(logit_of<BF>(key_in(pick.token)), top, set.inv_t) / end.mass);
   }
 }
 

@@ -74,7 +74,8 @@ def test_ties_and_orders(mk, dev):
     ramp = torch.stack([torch.arange(V), -torch.arange(V)]).float().repeat(4, 1) * 1e-3
     zero = torch.where(torch.rand(8, V, generator=g) < 0.5, 0.0, -0.0)
     u = torch.rand(8, generator=g)
-    for x in (few, ramp, zero, few.to(torch.bfloat16)):
+    small = (0.03 * torch.randn(8, V, generator=g)).to(torch.bfloat16)      # both signs in one bin
+    for x in (few, ramp, zero, few.to(torch.bfloat16), small, small.float()):
         for kw in (dict(), dict(top_k=7777), dict(top_p=0.7), dict(top_k=5001, top_p=0.3), dict(min_p=0.4), dict(temperature=0.05)):
             check(mk, dev, x, u, **kw)
 
