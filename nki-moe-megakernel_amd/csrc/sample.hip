@@ -69,20 +69,30 @@ MKD_DEV double mass_of(float l, float top, double inv_t) {
   if (top == INFINITY) return 0.0;
   return exp(((double)l - (double)top) * inv_t);
 }
-// the bin's place on the scale of z (monotone in l)
-MKD_DEV double place_of(float l, double inv_t) { return floor((double)l * inv_t * kSmRes); }
-// A token's weight from its place: the distance y from the bin's middle is within 1/32,
-// so six terms of the exponential series leave 2^-47; + 2^52 rounds to a whole number.
-MKD_DEV u64 weight_of(float l, double place, double inv_t) {
-  const double y = fma(place, -1.0 / kSmRes, (double)l * inv_t) - 0.5 / kSmRes;
-  double p = 1.0 / 720;
-  p = fma(p, y, 1.0 / 120);
-  p = fma(p, y, 1.0 / 24);
-  p = fma(p, y, 1.0 / 6);
-  p = fma(p, y, 0.5);
-  p = fma(p, y, 1.0);
-  p = fma(p, y, 1.0);
-  return __double_as_longlong(fma(p, kSmOne, 0x1p52)) & ((1ull << 52) - 1);
+// z in bins; its whole part is the bin's place (monotone in l)
+MKD_DEV double scaled(float l, double inv_t) { return (double)l * (inv_t * kSmRes); }
+MKD_DEV double place_of(float l, double inv_t) { return floor(scaled(l, inv_t)); }
+// A token's weight from its fraction f of a bin: exp((f - 1/2) / 16), whose series to the
+// fifth power (written out in powers of f) leaves 2^-39; + 2^52 rounds to a whole number.
+constexpr double sm_term(int k) {
+  double sum = 0.0, term = 1.0;                 // term: 1 / (16^m m!)
+  for (int m = 0; m <= 5; ++m) {
+    if (m > 0) term /= kSmRes * m;
+    if (m < k) continue;
+    double c = term;                            // times binomial(m, k) (-1/2)^(m - k)
+    for (int i = 0; i < m - k; ++i) c *= -0.5 * (m - i) / (i + 1);
+    sum += c;
+  }
+  return sum * kSmOne;
+}
+MKD_DEV u64 weight_of(double f) {
+  double p = sm_term(5);
+  p = fma(p, f, sm_term(4));
+  p = fma(p, f, sm_term(3));
+  p = fma(p, f, sm_term(2));
+  p = fma(p, f, sm_term(1));
+  p = fma(p, f, sm_term(0) + 0x1p52);
+  return __double_as_longlong(p) & ((1ull << 52) - 1);
 }
 // bit patterns in the order of the logits (a bf16 one's upper half); -0 and +0 are one value
 template <bool BF>
@@ -132,7 +142,7 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
 #pragma unroll
       for (int e = 0; e < G; ++e) {
         const float f = BF ? ((e & 1) ? bf_hi(v[e / 2]) : bf_lo(v[e / 2])) : __uint_as_float(v[e & 3]);
-        l[G * q + e] = f == f ? f : -INFINITY;
+        l[G * q + e] = fmaxf(f, -INFINITY);     // (a NaN: -inf)
       }
     } else {
 #pragma unroll
@@ -154,12 +164,12 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
 #pragma unroll
   for (int i = 0; i < kSmPer; ++i) {
     at[i] = kSmBins << 16;
-    const double place = place_of(l[i], s.inv_t), below = top_place - place;
-    // (below an infinite maximum everything is outside; -inf always is)
-    const bool same = l[i] == top;
-    if (!(same || below < kSmBins) || l[i] == -INFINITY) continue;
-    const int j = same ? 0 : (int)below;
-    const u64 add = (1ull << kSmMassBits) | (top == INFINITY ? (u64)kSmOne : weight_of(l[i], place, s.inv_t));
+    const double z = scaled(l[i], s.inv_t), place = floor(z);
+    double below = top_place - place;           // (-inf: infinitely far)
+    if (top == INFINITY) below = l[i] == top ? 0.0 : kSmBins;
+    if (!(below < kSmBins)) continue;
+    const u64 add = (1ull << kSmMassBits) | (top == INFINITY ? (u64)kSmOne : weight_of(z - place));
+    const int j = (int)below;
     at[i] = j << 16 | (uint32_t)(atomicAdd(&bins[j], add) >> kSmMassBits);
   }
   __syncthreads();
@@ -268,10 +278,25 @@ MKD_DEV unsigned count_of(SmShared& s, bool yes) {
   __syncthreads();
   return v;
 }
+// Up to 64 distinct numbers in rising order, one a lane (the others hold ~0), by one wave:
+// each lane's rank is the count of smaller ones.
+MKD_DEV u64 sort_wave(u64* buf, u64 v, unsigned n) {
+  const int lane = threadIdx.x & 63;
+  unsigned rank = 0;
+  for (unsigned i = 0; i < n; ++i) {
+    const u64 o = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 |
+                  (uint32_t)__builtin_amdgcn_readlane((int)v, i);
+    rank += o < v;
+  }
+  if (lane < (int)n) buf[rank] = v;
+  wave_lds_sync();
+  return lane < (int)n ? buf[lane] : ~0ull;
+}
 // Rising bitonic sort of one number per thread among the first `n` threads (the others
 // hold ~0): strides inside a wave by shuffles, longer ones through LDS.
 MKD_DEV u64 sort_up(SmShared& s, u64 v, unsigned n) {
   const unsigned x = threadIdx.x;
+  if (n <= 64) return x < 64 ? sort_wave(s.token, v, n) : v;
   for (unsigned size = 2; size / 2 < n; size <<= 1)
     for (unsigned stride = size >> 1; stride > 0; stride >>= 1) {
       u64 o;
@@ -308,8 +333,8 @@ struct SmRow {
 
   MKD_DEV u64 weight(uint32_t key) const {
     if (top == INFINITY) return (u64)kSmOne;
-    const float l = logit_of<BF>(key);
-    return weight_of(l, place_of(l, inv_t), inv_t);
+    const double z = scaled(logit_of<BF>(key), inv_t);
+    return weight_of(z - floor(z));
   }
   // member m of the staged bin: its index, and its logit's bit pattern
   MKD_DEV void member(unsigned m, uint32_t& key, uint32_t& index) const {
@@ -369,24 +394,32 @@ struct SmRow {
     __syncthreads();
     return s.first[nc];
   }
-  MKD_DEV void stage(int bin) {
-    if (staged == bin) return;
-    staged = bin;
-    n = locate(bin, bin);
-    uint32_t lo = 0xffffffffu, hi = 0u;
-    for (unsigned m = threadIdx.x; m < n; m += 8 * kSmRow) {
-      uint32_t key[8], index[8];
-      fetch<8>(m, key, index);
+  // this thread's members, N in flight, into LDS where they fit; their range in kmin, kmax
+  template <int N>
+  MKD_DEV void load() {
+    for (unsigned m = threadIdx.x; m < n; m += N * kSmRow) {
+      uint32_t key[N], index[N];
+      fetch<N>(m, key, index);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         if (n <= kSmStage && m + i * kSmRow < n) {
           s.key[m + i * kSmRow] = key[i];
           s.index[m + i * kSmRow] = index[i];
         }
-        lo = min(lo, key[i]);
-        hi = max(hi, key[i]);
+        kmin = min(kmin, key[i]);
+        kmax = max(kmax, key[i]);
       }
     }
+  }
+  MKD_DEV void stage(int bin) {
+    if (staged == bin) return;
+    staged = bin;
+    n = locate(bin, bin);
+    kmin = 0xffffffffu;
+    kmax = 0u;
+    if (n <= kSmRow) load<1>();
+    else load<8>();
+    uint32_t lo = kmin, hi = kmax;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
@@ -420,22 +453,12 @@ struct SmRow {
       if (x == 0) s.found = -1;
       __syncthreads();
       if (shift == 0) {
-        // one key a sub-bin: counted (few of them, ties among 16-bit logits, by a ballot each:
-        // thousands of atomics on a few words would queue), weighed once
-        for (unsigned m0 = 0; m0 < n; m0 += kSmRow) {
-          uint32_t key = 0, index, d = ~0u;
-          if (m0 + x < n) {
-            member(m0 + x, key, index);
-            d = kmax - key - base;
-          }
-          if (range < 32) {
-            for (uint32_t v = 0; v <= range; ++v) {
-              const u64 same = __ballot(d == v);
-              if (same && (x & 63) == 0) atomicAdd(&s.sub_n[v], (unsigned)__popcll(same));
-            }
-          } else if (d <= range) {
-            atomicAdd(&s.sub_n[d], 1u);
-          }
+        // one key a sub-bin: counted, and weighed once
+        for (unsigned m = x; m < n; m += kSmRow) {
+          uint32_t key, index;
+          member(m, key, index);
+          const uint32_t d = kmax - key - base;
+          if (d <= range) atomicAdd(&s.sub_n[d], 1u);
         }
       } else {
         for (unsigned m = x; m < n; m += kSmRow) {
@@ -488,7 +511,7 @@ struct SmRow {
     }
     __syncthreads();
     if (x < 64) {
-      const u64 t = sort_up(s, x < (int)left ? s.token[x] : ~0ull, left);
+      const u64 t = sort_wave(s.token, x < (int)left ? s.token[x] : ~0ull, left);
       const u64 own = x < (int)left ? weight(key_in(t)) : 0ull;
       u64 m = own;
 #pragma unroll
@@ -598,9 +621,9 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
           m += v[i] & ((1ull << kSmMassBits) - 1);
         }
     }
-    // exp(middle - z_max): both from the maximum's place, so that no large number is subtracted
+    // exp(middle - z_max)
     const double unit = top == INFINITY ? 1.0 / kSmOne
-        : exp(fma(top_place, 1.0 / kSmRes, -((double)top * set.inv_t)) + (0.5 - x) / kSmRes) / kSmOne;
+        : exp(((top_place - scaled(top, set.inv_t)) + (0.5 - x)) / kSmRes) / kSmOne;
     double sm = (double)m * unit;
     scan_nm(s, s.wave_d, sn, sm);
     s.cum_n[x] = sn;
