@@ -85,15 +85,22 @@ constexpr double sm_term(int k) {
   }
   return sum * kSmOne;
 }
-MKD_DEV u64 weight_of(double f) {
-  double p = sm_term(5);
-  p = fma(p, f, sm_term(4));
-  p = fma(p, f, sm_term(3));
-  p = fma(p, f, sm_term(2));
-  p = fma(p, f, sm_term(1));
-  p = fma(p, f, sm_term(0) + 0x1p52);
-  return __double_as_longlong(p) & ((1ull << 52) - 1);
-}
+struct SmSeries {                               // the coefficients, in scalar registers
+  double c[6];
+  MKD_DEV SmSeries() {
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      c[k] = sm_term(k) + (k == 0 ? 0x1p52 : 0.0);
+      asm("" : "+s"(c[k]));                     // (else every use moves two literals first)
+    }
+  }
+  MKD_DEV u64 weight(double f) const {
+    double p = c[5];
+#pragma unroll
+    for (int k = 4; k >= 0; --k) p = fma(p, f, c[k]);
+    return __double_as_longlong(p) & ((1ull << 52) - 1);
+  }
+};
 // bit patterns in the order of the logits (a bf16 one's upper half); -0 and +0 are one value
 template <bool BF>
 MKD_DEV uint32_t key_of(float l) {
@@ -122,7 +129,7 @@ MKD_DEV float logit_at(const mkd_sample_args& a, long long row, int i) {
 // (bf16: 8 x + 4096 (i / 8) + i % 8).
 template <bool BF, bool VEC>
 __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_args a, SmRecord* rec) {
-  __shared__ u64 bins[kSmBins];
+  __shared__ u64 bins[kSmBins + 32];            // (32 behind, for what lies outside: no branches)
   __shared__ unsigned first[kSmBins];
   __shared__ __attribute__((aligned(16))) uint16_t list[kSmChunk];
   __shared__ float wtop[kSmThreads / 64];
@@ -160,17 +167,23 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
   if (x == 0) r.top = top;
   if (top == -INFINITY) return;                 // nothing to choose here (the rest is not read)
   const double top_place = place_of(top, s.inv_t);
-  uint32_t at[kSmPer];                          // bin << 16 | place among its members
+  uint16_t bin[kSmPer];
+  uint32_t rank[kSmPer];                        // among its members
+  if (top < INFINITY) {
+    const SmSeries series;
 #pragma unroll
-  for (int i = 0; i < kSmPer; ++i) {
-    at[i] = kSmBins << 16;
-    const double z = scaled(l[i], s.inv_t), place = floor(z);
-    double below = top_place - place;           // (-inf: infinitely far)
-    if (top == INFINITY) below = l[i] == top ? 0.0 : kSmBins;
-    if (!(below < kSmBins)) continue;
-    const u64 add = (1ull << kSmMassBits) | (top == INFINITY ? (u64)kSmOne : weight_of(z - place));
-    const int j = (int)below;
-    at[i] = j << 16 | (uint32_t)(atomicAdd(&bins[j], add) >> kSmMassBits);
+    for (int i = 0; i < kSmPer; ++i) {
+      const double z = scaled(l[i], s.inv_t), place = floor(z);
+      const double below = top_place - place;   // (-inf: infinitely far)
+      const int j = (int)below;
+      bin[i] = (uint16_t)(j < kSmBins ? j : kSmBins + (x & 31));
+      rank[i] = (uint32_t)(atomicAdd(&bins[bin[i]], (1ull << kSmMassBits) | series.weight(z - place)) >> 32);
+    }
+  } else {                                      // infinite logits share the mass
+    for (int i = 0; i < kSmPer; ++i) {
+      bin[i] = l[i] == top ? 0 : kSmBins;
+      if (bin[i] < kSmBins) rank[i] = (uint32_t)(atomicAdd(&bins[0], (1ull << kSmMassBits) | (u64)kSmOne) >> 32);
+    }
   }
   __syncthreads();
   // exclusive scan of the counts, a bin a thread
@@ -198,8 +211,8 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSmPer; ++i)
-    if (at[i] >> 16 < kSmBins)
-      list[first[at[i] >> 16] + (at[i] & 0xffff)] = (uint16_t)(G * x + G * kSmThreads * (i / G) + i % G);
+    if (bin[i] < kSmBins)
+      list[first[bin[i]] + (rank[i] >> (kSmMassBits - 32))] = (uint16_t)(G * x + G * kSmThreads * (i / G) + i % G);
   __syncthreads();
   for (unsigned i = x * 8; i < total; i += kSmThreads * 8) st16(r.list + i, ld16(list + i));
 }
@@ -327,6 +340,7 @@ struct SmRow {
   int b, nc;
   float top;
   double inv_t;
+  SmSeries series{};
   int staged = -1;
   unsigned n = 0;                               // members of the staged bin
   uint32_t kmin = 0, kmax = 0;                  // their least and largest bit patterns
@@ -334,7 +348,7 @@ struct SmRow {
   MKD_DEV u64 weight(uint32_t key) const {
     if (top == INFINITY) return (u64)kSmOne;
     const double z = scaled(logit_of<BF>(key), inv_t);
-    return weight_of(z - floor(z));
+    return series.weight(z - floor(z));
   }
   // member m of the staged bin: its index, and its logit's bit pattern
   MKD_DEV void member(unsigned m, uint32_t& key, uint32_t& index) const {
