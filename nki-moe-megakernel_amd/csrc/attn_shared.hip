@@ -5,27 +5,31 @@
 // l, weighted values O) that join exactly: O = sum_c 2^(m_c - m) O_c, l alike.  So the
 // prefix of a group is attended once by a matrix of ALL its query rows (sequences x new
 // tokens x the kv head's query heads), each sequence's own positions by its own rows,
-// and one launch joins a row's partials:
-//   1. prefix: block (chunk of positions, kv head, tile of 16 QT rows of a group)
-//   2. own:    block (chunk, kv head, tile of 16 QT rows of a sequence)
-//   3. combine: one wave per row over its live chunks, the sink joined there
+// and a second launch joins a row's partials:
+//   1. units of both kinds in one grid, the prefixes' first: (chunk of positions, kv head,
+//      tile of a group's rows), and (chunk, kv head, tile of a sequence's rows)
+//   2. combine: one wave per row over its live chunks, the sink joined there
 //
-// In 1 and 2 wave w of 4 takes the chunk's 32-position steps w, w + 4, ..; per step
-// (two 16-row tiles of the cache)
+// Per 32-position step a wave with QT tiles of 16 query rows forms
 //   S = K . q^T   v_mfma_f32_16x16x32_bf16, A = 16 K rows, B = 16 query rows;
 //                 D lane l holds S[position 4 (l/16) + i][row l % 16]
-//   O += P . V    P straight from the S layout, V rows as they come (lane column
-//                 l % 16 owns D / 16 contiguous elements; d-tile dt is element dt)
+//   O += P . V    P straight from the S layout, V rows transposed on the way
 //   l += P . 1    the sum of the same rounded P, by one more MFMA
-// A K or V operand is loaded and formed once for the QT row tiles.  P is rounded to
-// bf16 for the matrix instruction (a relative 2^-9 of each term, the rounding of the
-// output itself); scores, maxima, l and O stay fp32.
+// P is rounded to bf16 for the matrix instruction (a relative 2^-9 of each term, the
+// rounding of the output itself); scores, maxima, l and O stay fp32.
+//
+// staged (more than 32 query rows): the block's 4 waves hold 16 QT rows each and share
+// the steps' K and V rows through a ring of three LDS stages filled asynchronously
+// (global_load_lds), one barrier a step.  direct (few rows, and every sequence's own
+// positions): the waves take steps of their own, rows straight to registers a step ahead,
+// and merge at the end: nothing to share, and no barrier to wait at.
 //
 // The rows' addresses are formed once per chunk in LDS, so blocks of any length may end
 // inside a tile; a position past the length or in no valid block reads a row of zeros
 // (so that what a page holds behind a sequence, NaN among it, never meets a product).
 #include "common.h"
 #include "mkd_internal.h"
+#include "coherent.h"
 
 namespace mkd {
 
@@ -80,98 +84,155 @@ MKD_DEV bool find_tile(const SharedArgs& a, int tile, int per, int r1, int lane,
 
 }  // namespace
 
-template <int D, int QT, bool FP8, bool PREFIX>
-__global__ void __launch_bounds__(64 * kShWaves, QT == 4 ? 1 : (QT == 2 ? 2 : 3))
-attn_shared_kernel(SharedArgs a) {
-  constexpr int EB = FP8 ? 1 : 2;               // bytes per cached element
-  constexpr int NK = D / 32, NDT = D / 16, ROWS = 16 * QT;
-  constexpr int KL = D * EB / 64;               // 16-byte loads of a lane's K row share
-  constexpr int VD = D * EB / 64;               // dwords of a lane's V row share
-  constexpr int kTab = 2 * kShMaxChunk * 8, kOut = kShWaves * ROWS * D * 4;
-  __shared__ __attribute__((aligned(16))) char mem[kTab > kOut ? kTab : kOut];
-  __shared__ float m_s[kShWaves][ROWS], l_s[kShWaves][ROWS];
-  long long* const koff = reinterpret_cast<long long*>(mem);   // (until the merge)
-  long long* const voff = koff + kShMaxChunk;
-  float* const o_s = reinterpret_cast<float*>(mem);
-  const int lane = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int q4 = lane >> 4, col = lane & 15;
-  const int gqa = a.p.nq / a.p.nkv, S = a.p.s_tkg, r1 = S * gqa;
-  const int c = blockIdx.x / a.p.nkv, kvh = blockIdx.x % a.p.nkv;
+namespace {
 
-  // ---- this block's rows, table and length ----
-  int b0, row0, nrow, len, width;
+constexpr int kShStages = 3;                    // LDS ring of the staged form
+
+// One unit: `nrow` query rows (from row0 of the sequences from b0 on) against the
+// positions [chunk0, min(chunk0 + CP, len)) of one table, as partial `slot`.
+struct Unit {
   const int* table;
-  if constexpr (PREFIX) {
-    if (c >= a.prefix_chunks) return;
-    int g, first;
-    if (!find_tile(a, blockIdx.y, ROWS, r1, lane, g, first)) return;
-    b0 = min(max(a.p.prefix_starts[g], 0), a.p.B);
-    row0 = first * ROWS;
-    nrow = (min(max(a.p.prefix_starts[g + 1], b0), a.p.B) - b0) * r1 - row0;
-    width = a.p.prefix_blocks;
-    table = a.p.prefix_tables + (long long)g * width;
-    len = a.p.prefix_lens[g];
-  } else {
-    b0 = blockIdx.z;
-    row0 = blockIdx.y * ROWS;
-    nrow = r1 - row0;
-    width = a.p.own_blocks;
-    table = a.p.tables + (long long)b0 * width;
-    len = a.p.lens[b0];
-  }
-  len = __builtin_amdgcn_readfirstlane(min(max(len, 0), width * a.p.block_len));
-  b0 = __builtin_amdgcn_readfirstlane(b0);
-  row0 = __builtin_amdgcn_readfirstlane(row0);
-  nrow = __builtin_amdgcn_readfirstlane(min(nrow, ROWS));
-  const int CP = PREFIX ? a.prefix_chunk : a.own_chunk, chunk0 = c * CP;
-  if (chunk0 >= len) return;                    // whole block
-  const int nst = (min(CP, len - chunk0) + kShStep - 1) / kShStep;
+  int b0, row0, nrow, len, chunk0, CP, kvh, slot, width;
+  bool own;                                     // new token i sees len - (S - 1 - i) positions
+};
 
-  // ---- byte offsets of the chunk's rows, -1: a row of zeros ----
-  for (int i = threadIdx.x; i < nst * kShStep; i += 64 * kShWaves) {
-    const int t = chunk0 + i;
+// Query rows of the unit as B operands: lane's row 16 t + col, head element 32 kk + 8 q4
+// (FP8: q4 D/4 + 8 kk, as a lane's K bytes lie).  A negative scale goes to the queries'
+// signs, so that the largest product is the largest score.
+template <int D, int QT, bool FP8>
+MKD_DEV void load_q(const SharedArgs& a, const Unit& u, int first, u32x4_t (&qf)[QT][D / 32], int (&lim)[QT]) {
+  const int lane = threadIdx.x & 63, q4 = lane >> 4, col = lane & 15;
+  const int gqa = a.p.nq / a.p.nkv, S = a.p.s_tkg, r1 = S * gqa;
+  const uint16_t* qp = static_cast<const uint16_t*>(a.p.q);
+  const uint32_t flip = a.p.softmax_scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = first + 16 * t + col, rr = u.row0 + min(r, u.nrow - 1);
+    const int b = u.b0 + rr / r1, s = (rr / gqa) % S, h = u.kvh * gqa + rr % gqa;
+    const uint16_t* src = qp + b * a.p.q_stride[0] + s * a.p.q_stride[1] + h * a.p.q_stride[2];
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+      const u32x4_t v = ld16(src + (FP8 ? q4 * (D / 4) + 8 * kk : 32 * kk + 8 * q4));
+      qf[t][kk] = r < u.nrow ? v ^ u32x4_t{flip, flip, flip, flip} : u32x4_t{0u, 0u, 0u, 0u};
+    }
+    lim[t] = u.own ? u.len - (S - 1 - s) : u.len;
+  }
+}
+// Byte offsets of the chunk's rows in the caches, -1: a row of zeros.
+MKD_DEV void fill_offsets(const SharedArgs& a, const Unit& u, int eb, int n, long long* koff, long long* voff) {
+  for (int i = threadIdx.x; i < n; i += 64 * kShWaves) {
+    const int t = u.chunk0 + i;
     long long k = -1, v = -1;
-    if (t < len) {
-      const int blk = table[t / a.p.block_len], r = t % a.p.block_len;
+    if (t < u.len) {
+      const int blk = u.table[t / a.p.block_len], r = t % a.p.block_len;
       if ((unsigned)blk < (unsigned)a.p.num_blocks) {
-        k = (blk * a.p.k_cache_stride[0] + r * a.p.k_cache_stride[1] + kvh * a.p.k_cache_stride[2]) * EB;
-        v = (blk * a.p.v_cache_stride[0] + r * a.p.v_cache_stride[1] + kvh * a.p.v_cache_stride[2]) * EB;
+        k = (blk * a.p.k_cache_stride[0] + r * a.p.k_cache_stride[1] + u.kvh * a.p.k_cache_stride[2]) * eb;
+        v = (blk * a.p.v_cache_stride[0] + r * a.p.v_cache_stride[1] + u.kvh * a.p.v_cache_stride[2]) * eb;
       }
     }
     koff[i] = k;
     voff[i] = v;
   }
+}
+MKD_DEV gptr row_at(const void* cache, long long off) {
+  return (gptr)(off < 0 ? reinterpret_cast<const char*>(g_zero_row) : static_cast<const char*>(cache) + off);
+}
 
-  // ---- the tile's queries: B operands, head element 32 kk + 8 q4 (FP8: q4 D/4 + 8 kk) ----
-  u32x4_t qf[QT][NK];
-  int lim[QT];                                  // positions that row 16 t + col sees
-  const uint16_t* qp = static_cast<const uint16_t*>(a.p.q);
+// The running softmax of one wave's rows: scores of a step to probabilities, and what
+// they leave of the sums so far.
+template <int QT, int NDT>
+struct Rows {
+  f32x4_t o[QT][NDT], l[QT];                    // rows 4 q4 + i of tile t
+  float m[QT];                                  // row col of tile t, in units of log2
+  MKD_DEV Rows() {
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = 16 * t + col, rr = row0 + min(r, nrow - 1);
-    const int b = b0 + rr / r1, s = (rr / gqa) % S, h = kvh * gqa + rr % gqa;
-    const uint16_t* src = qp + b * a.p.q_stride[0] + s * a.p.q_stride[1] + h * a.p.q_stride[2];
+    for (int t = 0; t < QT; ++t) {
+      m[t] = -INFINITY;
+      l[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const u32x4_t v = ld16(src + (FP8 ? q4 * (D / 4) + 8 * kk : 32 * kk + 8 * q4));
-      qf[t][kk] = r < nrow ? v : u32x4_t{0u, 0u, 0u, 0u};
+      for (int dt = 0; dt < NDT; ++dt) o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    lim[t] = PREFIX ? len : len - (S - 1 - s);
   }
-  const int lim_min = PREFIX ? len : len - (S - 1);
-  const float scale2 = a.p.softmax_scale * kLog2e;
+  // raw products sc of tile t (times scale2: scores); its P operand
+  MKD_DEV u32x4_t weigh(int t, const f32x4_t (&sc)[2], float scale2) {
+    const int q4 = (threadIdx.x & 63) >> 4;
+    float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+    mx = fmaxf(mx, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
+    const float mn = fmaxf(m[t], mx);
+    if (__any(mn > m[t])) {                     // uniform: a maximum moved
+      const float alpha = m[t] == -INFINITY ? 0.f : exp2_hw(m[t] - mn);
+      m[t] = mn;
+      float al[4];                              // (o and l rows are 4 q4 + i)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * q4 + i, 64);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[t][i] *= al[i];
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][dt][i] *= al[i];
+    }
+    const float ms = m[t] == -INFINITY ? 0.f : m[t];
+    u32x4_t ph;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = exp2_hw(fmaf(sc[u][i], scale2, -ms));
+      ph[2 * u] = pack2bf(p[0], p[1]);
+      ph[2 * u + 1] = pack2bf(p[2], p[3]);
+    }
+    l[t] = mfma16x16x32(ph, u32x4_t{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, l[t]);
+    return ph;
+  }
+};
+// positions that row `lim` does not see
+MKD_DEV void hide(f32x4_t (&sc)[2], int p0, int lim) {
+  const int q4 = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (p0 + 16 * u + 4 * q4 + i >= lim) sc[u][i] = -INFINITY;
+}
+MKD_DEV float scale_log2(const SharedArgs& a) {   // (0: small enough, and -inf stays -inf)
+  return fmaxf(fabsf(a.p.softmax_scale) * kLog2e, 1e-37f);
+}
+MKD_DEV long long part_at(const SharedArgs& a, const Unit& u, int r) {   // the unit's row r
+  const int gqa = a.p.nq / a.p.nkv, S = a.p.s_tkg, r1 = S * gqa, rr = u.row0 + r;
+  return (((long long)(u.b0 + rr / r1) * S + (rr / gqa) % S) * a.p.nq + u.kvh * gqa + rr % gqa) * a.slots + u.slot;
+}
+
+// ---- direct: position steps w, w + 4, .. to wave w, the waves merged at the end ----
+template <int D, int QT, bool FP8>
+MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (*m_s)[32], float (*l_s)[32]) {
+  constexpr int EB = FP8 ? 1 : 2;               // bytes per cached element
+  constexpr int NK = D / 32, NDT = D / 16, ROWS = 16 * QT;
+  constexpr int KL = D * EB / 64;               // 16-byte loads of a lane's K row share
+  constexpr int VD = D * EB / 64;               // dwords of a lane's V row share
+  long long* const koff = reinterpret_cast<long long*>(mem);
+  long long* const voff = koff + kShMaxChunk;
+  float* const o_s = reinterpret_cast<float*>(mem);
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q4 = lane >> 4, col = lane & 15;
+  const int nst = (min(un.CP, un.len - un.chunk0) + kShStep - 1) / kShStep;
+  u32x4_t qf[QT][NK];
+  int lim[QT];
+  load_q<D, QT, FP8>(a, un, 0, qf, lim);
+  fill_offsets(a, un, EB, nst * kShStep, koff, voff);
+  const int lim_min = un.own ? un.len - (a.p.s_tkg - 1) : un.len;
+  const float scale2 = scale_log2(a);
   __syncthreads();
 
-  const char* const kc = static_cast<const char*>(a.p.k_cache);
-  const char* const vc = static_cast<const char*>(a.p.v_cache);
   u32x4_t kr[2][KL];
   uint32_t vr[2][4][VD];
   auto load_k = [&](int st) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const long long off = koff[st * kShStep + 16 * u + col];
-      const gptr p = (gptr)(off < 0 ? reinterpret_cast<const char*>(g_zero_row) : kc + off);
+      const gptr p = row_at(a.p.k_cache, koff[st * kShStep + 16 * u + col]);
 #pragma unroll
       for (int j = 0; j < KL; ++j) kr[u][j] = g_ld16(p + (FP8 ? q4 * (D / 4) + 16 * j : q4 * 16 + 64 * j));
     }
@@ -181,8 +242,7 @@ attn_shared_kernel(SharedArgs a) {
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const long long off = voff[st * kShStep + 16 * u + 4 * q4 + j];
-        const gptr p = (gptr)(off < 0 ? reinterpret_cast<const char*>(g_zero_row) : vc + off) + col * (4 * VD);
+        const gptr p = row_at(a.p.v_cache, voff[st * kShStep + 16 * u + 4 * q4 + j]) + col * (4 * VD);
         if constexpr (VD == 4) {
           const u32x4_t v = g_ld16(p);
 #pragma unroll
@@ -196,27 +256,15 @@ attn_shared_kernel(SharedArgs a) {
         }
       }
   };
-
-  f32x4_t o[QT][NDT], l[QT];
-  float m[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    m[t] = -INFINITY;
-    l[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-  const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-
+  Rows<QT, NDT> rows;
   int st = w;
   if (st < nst) {
     load_k(st);
     load_v(st);
   }
   for (; st < nst; st += kShWaves) {
-    const int p0 = chunk0 + st * kShStep, sn = st + kShWaves;
-    // ---- scores, in units of log2 ----
-    float sc[QT][2][4];
+    const int p0 = un.chunk0 + st * kShStep, sn = st + kShWaves;
+    f32x4_t sc[QT][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       u32x4_t kf[NK];
@@ -227,59 +275,21 @@ attn_shared_kernel(SharedArgs a) {
       }
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+        sc[t][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) acc = mfma16x16x32(kf[kk], qf[t][kk], acc);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[t][u][i] = acc[i] * scale2;
+        for (int kk = 0; kk < NK; ++kk) sc[t][u] = mfma16x16x32(kf[kk], qf[t][kk], sc[t][u]);
       }
     }
     if (sn < nst) load_k(sn);
-    if (p0 + kShStep > lim_min) {               // (uniform) positions some row does not see
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (p0 + 16 * u + 4 * q4 + i >= lim[t]) sc[t][u][i] = -INFINITY;
-    }
-    // ---- online softmax per row (the four lanes sharing col) ----
     u32x4_t ph[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      float mx = sc[t][0][0];
-#pragma unroll
-      for (int k = 1; k < 8; ++k) mx = fmaxf(mx, sc[t][k >> 2][k & 3]);
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m[t], mx);
-      if (__any(mn > m[t])) {                   // uniform: a maximum moved
-        const float alpha = m[t] == -INFINITY ? 0.f : exp2_hw(m[t] - mn);
-        m[t] = mn;
-        float al[4];                            // (o and l rows are 4 q4 + i)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * q4 + i, 64);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l[t][i] *= al[i];
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][dt][i] *= al[i];
-      }
-      const float ms = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = exp2_hw(sc[t][u][i] - ms);
-        ph[t][2 * u] = pack2bf(p[0], p[1]);
-        ph[t][2 * u + 1] = pack2bf(p[2], p[3]);
-      }
-      l[t] = mfma16x16x32(ph[t], ones, l[t]);
+      if (p0 + kShStep > lim_min) hide(sc[t], p0, lim[t]);
+      ph[t] = rows.weigh(t, sc[t], scale2);
     }
-    // ---- P . V: the operand's 16-bit halves from two V rows by one byte permute per
-    // dword (selector 0x05040100: bytes 0-1 of each row; 0x07060302: bytes 2-3) ----
+    // P . V: lane column col owns the NDT contiguous elements of its V rows, d-tile dt is
+    // element dt; the operand's 16-bit halves from two rows by one byte permute per dword
+    // (selector 0x05040100: bytes 0-1 of each row; 0x07060302: bytes 2-3)
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
       u32x4_t bop;
@@ -302,29 +312,27 @@ attn_shared_kernel(SharedArgs a) {
         }
       }
 #pragma unroll
-      for (int t = 0; t < QT; ++t) o[t][dt] = mfma16x16x32(ph[t], bop, o[t][dt]);
+      for (int t = 0; t < QT; ++t) rows.o[t][dt] = mfma16x16x32(ph[t], bop, rows.o[t][dt]);
     }
     if (sn < nst) load_v(sn);
   }
-
   // ---- merge the waves into this chunk's partial ----
   __syncthreads();                              // the offsets are read; o_s takes their place
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    if (lane < 16) m_s[w][16 * t + lane] = m[t];
+    if (lane < 16) m_s[w][16 * t + lane] = rows.m[t];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * t + 4 * q4 + i;
-      if (col == 0) l_s[w][r] = l[t][i];
+      if (col == 0) l_s[w][r] = rows.l[t][i];
 #pragma unroll
       for (int q = 0; q < NDT / 4; ++q)
         *reinterpret_cast<f32x4_t*>(o_s + ((w * ROWS + r) * D + col * NDT + 4 * q)) =
-            f32x4_t{o[t][4 * q][i], o[t][4 * q + 1][i], o[t][4 * q + 2][i], o[t][4 * q + 3][i]};
+            f32x4_t{rows.o[t][4 * q][i], rows.o[t][4 * q + 1][i], rows.o[t][4 * q + 2][i], rows.o[t][4 * q + 3][i]};
     }
   }
   __syncthreads();
-  const int slot = PREFIX ? c : a.prefix_chunks + c;
-  for (int idx = threadIdx.x * 4; idx < nrow * D; idx += 64 * kShWaves * 4) {
+  for (int idx = threadIdx.x * 4; idx < un.nrow * D; idx += 64 * kShWaves * 4) {
     const int r = idx / D, d = idx % D;
     float M = -INFINITY;
 #pragma unroll
@@ -337,12 +345,247 @@ attn_shared_kernel(SharedArgs a) {
       L += l_s[q][r] * f;
       O += *reinterpret_cast<const f32x4_t*>(o_s + ((q * ROWS + r) * D + d)) * f;
     }
-    const int rr = row0 + r;
-    const long long row = ((long long)(b0 + rr / r1) * S + (rr / gqa) % S) * a.p.nq + kvh * gqa + rr % gqa;
-    const long long at = row * a.slots + slot;
+    const long long at = part_at(a, un, r);
     *reinterpret_cast<f32x4_t*>(a.part_o + at * D + d) = O;
     if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{M, L};
   }
+}
+
+// Wrappers outside the templates.
+MKD_DEV void g_to_lds16(gptr src, char* dst) {   // lane l's 16 bytes to dst + 16 l (dst uniform)
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+// Four 16-bit values of one column: per 16 lanes a tile of 4 rows x 16, lane i naming the
+// 8 bytes of row i / 4 and columns 4 (i % 4) .., lane j getting column j.
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
+MKD_DEV uint2 lds_tr8(const char* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p));
+}
+template <int N>
+MKD_DEV void wait_loads() {                     // all but the last N vector memory accesses
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+// ---- staged: wave w holds rows 16 QT w .., every step's K and V rows through LDS ----
+// A stage holds 32 K rows, then 32 V rows, in pieces of 16 bytes; piece p of row r is the
+// row's piece p ^ r (modulo the pieces of a row), so that the 16 rows of an operand read
+// lie on different banks.
+template <int D, int QT, bool FP8>
+MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
+  constexpr int EB = FP8 ? 1 : 2, NK = D / 32, NDT = D / 16;
+  constexpr int RB = D * EB, CPR = RB / 16;     // bytes, pieces of a row
+  constexpr int kStage = 2 * kShStep * RB, CPW = CPR / kShWaves;   // 1 KiB copies per wave and stage
+  static_assert(CPW >= 1, "a copy per wave");
+  char* const ring = mem;
+  long long* const koff = reinterpret_cast<long long*>(mem + kShStages * kStage);
+  long long* const voff = koff + kShMaxChunk;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q4 = lane >> 4, col = lane & 15;
+  const int nst = (min(un.CP, un.len - un.chunk0) + kShStep - 1) / kShStep;
+  const int first = 16 * QT * w;                // this wave's rows
+  u32x4_t qf[QT][NK];
+  int lim[QT];
+  load_q<D, QT, FP8>(a, un, first, qf, lim);
+  fill_offsets(a, un, EB, nst * kShStep, koff, voff);
+  const float scale2 = scale_log2(a);
+  __syncthreads();
+  auto copy = [&](int st) {
+    char* const dst = ring + (st % kShStages) * kStage;
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) {
+      const int n = w * CPW + i;                // (uniform) the stage's n-th KiB: K in the first half
+      const bool v = n >= CPR / 2;
+      const int piece = (v ? n - CPR / 2 : n) * 64 + lane, row = piece / CPR, p = piece % CPR;
+      const gptr src = row_at(v ? a.p.v_cache : a.p.k_cache, (v ? voff : koff)[st * kShStep + row]);
+      g_to_lds16(src + ((p ^ (row & (CPR - 1))) << 4), dst + n * 1024);
+    }
+  };
+  copy(0);
+  if (nst > 1) copy(1);
+  Rows<QT, NDT> rows;
+  const bool live = first < un.nrow;            // (uniform)
+  // operand reads: K row 16 u + col, V rows 16 u + 4 q4 + ..
+  const int kx = (col & (CPR - 1)) << 4;
+  const int vrow = 4 * q4 + (col >> 2), vx = (vrow & (CPR - 1)) << 4;
+  for (int st = 0; st < nst; ++st) {
+    if (st + 1 < nst) wait_loads<CPW>();        // stage st landed: this wave's part ..
+    else wait_loads<0>();
+    lds_barrier();                              // .. and everyone's; stage st - 1 is read
+    if (st + 2 < nst) copy(st + 2);
+    if (!live) continue;
+    const char* const ks = ring + (st % kShStages) * kStage;
+    const char* const vs = ks + kShStep * RB;
+    const int p0 = un.chunk0 + st * kShStep;
+    f32x4_t sc[QT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      u32x4_t kf[NK];
+      if constexpr (FP8) {
+#pragma unroll
+        for (int j = 0; j < RB / 64; ++j) {
+          const u32x4_t v = ld16(ks + (16 * u + col) * RB + ((((RB / 64) * q4 + j) << 4) ^ kx));
+          kf[2 * j] = codes_to_bf16(v[0], v[1]);
+          kf[2 * j + 1] = codes_to_bf16(v[2], v[3]);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) kf[kk] = ld16(ks + (16 * u + col) * RB + (((4 * kk + q4) << 4) ^ kx));
+      }
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        sc[t][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) sc[t][u] = mfma16x16x32(kf[kk], qf[t][kk], sc[t][u]);
+      }
+    }
+    u32x4_t ph[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      if (p0 + kShStep > un.len) hide(sc[t], p0, un.len);
+      ph[t] = rows.weigh(t, sc[t], scale2);
+    }
+    if constexpr (FP8) {
+      // lane column col owns NDT contiguous elements (one byte each) of its V rows
+      uint32_t vr[2][4][NDT / 4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = 16 * u + 4 * q4 + j, byte = col * NDT;
+          const char* p = vs + row * RB + ((byte & ~15) ^ ((row & (CPR - 1)) << 4)) + (byte & 15);
+#pragma unroll
+          for (int e = 0; e < NDT / 4; ++e) vr[u][j][e] = reinterpret_cast<const uint32_t*>(p)[e];
+        }
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        u32x4_t bop;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x2_t v = (dt & 2) ? cvt2_hi(vr[u][j][dt >> 2]) : cvt2_lo(vr[u][j][dt >> 2]);
+            x[j] = v[dt & 1];
+          }
+          bop[2 * u] = pack2bf(x[0], x[1]);
+          bop[2 * u + 1] = pack2bf(x[2], x[3]);
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) rows.o[t][dt] = mfma16x16x32(ph[t], bop, rows.o[t][dt]);
+      }
+    } else {
+      // d-tile dt is the elements 16 dt + col, transposed by the read itself
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        u32x4_t bop;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint2 v = lds_tr8(vs + (16 * u + vrow) * RB + (((2 * dt + ((col >> 1) & 1)) << 4) ^ vx) + (col & 1) * 8);
+          bop[2 * u] = v.x;
+          bop[2 * u + 1] = v.y;
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) rows.o[t][dt] = mfma16x16x32(ph[t], bop, rows.o[t][dt]);
+      }
+    }
+  }
+  // ---- the wave's rows out, through LDS in the order of the head's elements ----
+  __syncthreads();                              // every stage and offset is read
+  if (!live) return;
+  float* const o_s = reinterpret_cast<float*>(mem) + w * 16 * D;   // 16 rows at a time
+  const int n = min(un.nrow - first, 16 * QT);
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o_s[(4 * q4 + i) * D + (FP8 ? col * NDT + dt : 16 * dt + col)] = rows.o[t][dt][i];
+    wave_lds_sync();
+    for (int idx = lane * 4; idx < 16 * D; idx += 256) {
+      const int r = 16 * t + idx / D;
+      if (r < n)
+        *reinterpret_cast<f32x4_t*>(a.part_o + part_at(a, un, first + r) * D + idx % D) =
+            *reinterpret_cast<const f32x4_t*>(o_s + idx);
+    }
+    wave_lds_sync();
+    // row 4 q4 + i: its sum from lane column 0, its maximum from lane column 4 q4 + i
+    float mx[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx[i] = __shfl(rows.m[t], 4 * q4 + i, 64);
+    if (col == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * t + 4 * q4 + i;
+        if (r < n) *reinterpret_cast<float2*>(a.part_ml + part_at(a, un, first + r) * 2) = float2{mx[i], rows.l[t][i]};
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// PQ: 16-row tiles per wave of the staged prefixes, 0: prefixes direct; OQ: tiles of the
+// direct units.
+template <int D, bool FP8, int PQ, int OQ>
+__global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArgs a) {
+  constexpr int EB = FP8 ? 1 : 2, kTab = 2 * kShMaxChunk * 8;
+  constexpr int kDirect = kShWaves * 16 * OQ * D * 4 > kTab ? kShWaves * 16 * OQ * D * 4 : kTab;
+  constexpr int kStaged = PQ > 0 ? kShStages * 2 * kShStep * D * EB + kTab : 0;
+  constexpr int kMem = kDirect > kStaged ? kDirect : kStaged;
+  static_assert(kMem >= kShWaves * 16 * D * 4, "a wave's 16 rows out");
+  __shared__ __attribute__((aligned(1024))) char mem[kMem];
+  __shared__ float m_s[kShWaves][32], l_s[kShWaves][32];
+  const int r1 = a.p.s_tkg * (a.p.nq / a.p.nkv);
+  int L = blockIdx.x;
+  Unit u;
+  if (L < a.prefix_units) {
+    // the tiles of one (chunk, kv head) on one XCD (workgroups go round-robin by index)
+    constexpr int per = PQ > 0 ? kShWaves * 16 * PQ : 16 * OQ;
+    const int cell = L / (8 * a.prefix_tiles) * 8 + L % 8, tile = L / 8 % a.prefix_tiles;
+    const int c = cell / a.p.nkv;
+    if (c >= a.prefix_chunks) return;
+    int g, first;
+    if (!find_tile(a, tile, per, r1, threadIdx.x & 63, g, first)) return;
+    const int lo = min(max(a.p.prefix_starts[g], 0), a.p.B), hi = min(max(a.p.prefix_starts[g + 1], lo), a.p.B);
+    u.own = false;
+    u.b0 = lo;
+    u.row0 = first * per;
+    u.nrow = min((hi - lo) * r1 - u.row0, per);
+    u.width = a.p.prefix_blocks;
+    u.table = a.p.prefix_tables + (long long)g * u.width;
+    u.len = a.p.prefix_lens[g];
+    u.kvh = cell % a.p.nkv;
+    u.slot = c;
+    u.CP = a.prefix_chunk;
+  } else {
+    L -= a.prefix_units;
+    const int c = L % a.own_chunks, rest = L / a.own_chunks, tile = rest / a.p.nkv % a.own_tiles;
+    u.own = true;
+    u.kvh = rest % a.p.nkv;
+    u.b0 = rest / a.p.nkv / a.own_tiles;
+    u.row0 = tile * 16 * OQ;
+    u.nrow = min(r1 - u.row0, 16 * OQ);
+    u.width = a.p.own_blocks;
+    u.table = a.p.tables + (long long)u.b0 * u.width;
+    u.len = a.p.lens[u.b0];
+    u.slot = a.prefix_chunks + c;
+    u.CP = a.own_chunk;
+  }
+  u.chunk0 = (u.own ? u.slot - a.prefix_chunks : u.slot) * u.CP;
+  u.len = __builtin_amdgcn_readfirstlane(min(max(u.len, 0), u.width * a.p.block_len));
+  u.b0 = __builtin_amdgcn_readfirstlane(u.b0);
+  u.row0 = __builtin_amdgcn_readfirstlane(u.row0);
+  u.nrow = __builtin_amdgcn_readfirstlane(u.nrow);
+  if (u.chunk0 >= u.len) return;                // whole block
+  if constexpr (PQ > 0) {
+    if (!u.own) {
+      staged_unit<D, PQ, FP8>(a, u, mem);
+      return;
+    }
+  }
+  direct_unit<D, OQ, FP8>(a, u, mem, m_s, l_s);
 }
 
 // One wave per query row: its group's live prefix chunks, its own live chunks, the sink.
@@ -388,15 +631,15 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
   else dst[lane] = (uint16_t)f2bf(o[0] * inv);
 }
 
-// Shapes alone decide the split (lengths stay on the device): see SharedPlan.
+// Shapes alone decide the split (lengths stay on the device).
 SharedPlan shared_plan(const mkd_shared_prefix_args& p) {
   SharedPlan s{};
   const long long r1 = (long long)p.s_tkg * (p.nq / p.nkv), rows = r1 * p.B;
   const long long plen = p.G > 0 ? (long long)p.prefix_blocks * p.block_len : 0, olen = (long long)p.own_blocks * p.block_len;
-  s.prefix_qt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
-  s.own_qt = r1 <= 16 ? 1 : (r1 <= 32 ? 2 : 4);
+  s.prefix_qt = rows <= 32 ? 0 : (rows <= 64 ? 1 : 2);
+  s.own_qt = (rows <= 32 ? rows : r1) <= 16 ? 1 : 2;
   s.own_tiles = (int)((r1 + 16 * s.own_qt - 1) / (16 * s.own_qt));
-  const int per = 16 * s.prefix_qt;
+  const int per = s.prefix_qt ? 16 * kShWaves * s.prefix_qt : 16 * s.own_qt;
   s.prefix_tiles = p.G > 0 ? (rows + per - 1) / per + p.G - 1 : 0;
   auto chunk_for = [](long long len, long long units, long long want) {   // positions per block
     long long n = units > 0 ? (want + units - 1) / units : 1;              // chunks wanted
@@ -404,30 +647,30 @@ SharedPlan shared_plan(const mkd_shared_prefix_args& p) {
     c = (c + 127) / 128 * 128;
     return (int)(c < 128 ? 128 : (c > kShMaxChunk ? kShMaxChunk : c));
   };
-  s.prefix_chunk = chunk_for(plen, s.prefix_tiles * p.nkv, s.prefix_qt == 4 ? 256 : 768);
+  s.prefix_chunk = chunk_for(plen, s.prefix_tiles * p.nkv, 512);
   s.own_chunk = chunk_for(olen, (long long)p.B * s.own_tiles * p.nkv, 1024);
   s.prefix_chunks = (plen + s.prefix_chunk - 1) / s.prefix_chunk;
   s.own_chunks = (olen + s.own_chunk - 1) / s.own_chunk;
+  s.prefix_units = (s.prefix_chunks * p.nkv + 7) / 8 * 8 * s.prefix_tiles;
+  s.own_units = s.own_chunks * p.nkv * s.own_tiles * p.B;
   return s;
 }
 
 namespace {
 
-template <int D, bool FP8, bool PREFIX>
-void shared_rows(const SharedArgs& a, int qt, dim3 grid, hipStream_t s) {
-  switch (qt) {
-    case 1: hipLaunchKernelGGL((attn_shared_kernel<D, 1, FP8, PREFIX>), grid, dim3(64 * kShWaves), 0, s, a); break;
-    case 2: hipLaunchKernelGGL((attn_shared_kernel<D, 2, FP8, PREFIX>), grid, dim3(64 * kShWaves), 0, s, a); break;
-    default: hipLaunchKernelGGL((attn_shared_kernel<D, 4, FP8, PREFIX>), grid, dim3(64 * kShWaves), 0, s, a);
-  }
-}
 template <int D, bool FP8>
 void shared_run(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
-  // (units of one chunk and kv head on one XCD: x, a multiple of 8, runs fastest)
-  if (p.prefix_tiles > 0 && p.prefix_chunks > 0)
-    shared_rows<D, FP8, true>(a, p.prefix_qt, dim3((unsigned)((p.prefix_chunks * a.p.nkv + 7) / 8 * 8), (unsigned)p.prefix_tiles), s);
-  if (p.own_chunks > 0)
-    shared_rows<D, FP8, false>(a, p.own_qt, dim3((unsigned)(p.own_chunks * a.p.nkv), p.own_tiles, a.p.B), s);
+  const dim3 grid((unsigned)(p.prefix_units + p.own_units)), block(64 * kShWaves);
+  if (grid.x > 0) {
+    switch (p.prefix_qt * 2 + p.own_qt) {
+      case 1: hipLaunchKernelGGL((attn_shared_kernel<D, FP8, 0, 1>), grid, block, 0, s, a); break;
+      case 2: hipLaunchKernelGGL((attn_shared_kernel<D, FP8, 0, 2>), grid, block, 0, s, a); break;
+      case 3: hipLaunchKernelGGL((attn_shared_kernel<D, FP8, 1, 1>), grid, block, 0, s, a); break;
+      case 4: hipLaunchKernelGGL((attn_shared_kernel<D, FP8, 1, 2>), grid, block, 0, s, a); break;
+      case 5: hipLaunchKernelGGL((attn_shared_kernel<D, FP8, 2, 1>), grid, block, 0, s, a); break;
+      default: hipLaunchKernelGGL((attn_shared_kernel<D, FP8, 2, 2>), grid, block, 0, s, a);
+    }
+  }
   const long long rows = (long long)a.p.B * a.p.s_tkg * a.p.nq;
   hipLaunchKernelGGL(attn_shared_combine_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
 }

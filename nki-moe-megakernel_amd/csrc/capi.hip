@@ -1987,9 +1987,8 @@ static int check_shared(const mkd_shared_prefix_args* a) {
               MKD_ERR_INVALID, "attention_shared_prefix: %d groups of %d blocks, %d own blocks of %d rows", a->G,
               a->prefix_blocks, a->own_blocks, a->block_len);
   const SharedPlan p = shared_plan(*a);
-  MKD_REQUIRE((a->B == 0 || p.prefix_tiles <= 65535) && p.prefix_chunks * a->nkv < (1LL << 30) &&
-                  p.own_chunks * a->nkv < (1LL << 30) && (long long)a->B * a->s_tkg * a->nq < (1LL << 31),
-              MKD_ERR_UNSUPPORTED, "attention_shared_prefix: too many row tiles (%lld) or positions for one call", p.prefix_tiles);
+  MKD_REQUIRE(p.prefix_units + p.own_units < (1LL << 31) && (long long)a->B * a->s_tkg * a->nq < (1LL << 31),
+              MKD_ERR_UNSUPPORTED, "attention_shared_prefix: %lld units of work for one call", p.prefix_units + p.own_units);
   return MKD_OK;
 }
 
@@ -2022,6 +2021,10 @@ int mkd_attention_shared_prefix(const mkd_shared_prefix_args* a, void* workspace
   s.prefix_chunk = p.prefix_chunk;
   s.own_chunk = p.own_chunk;
   s.prefix_chunks = (int)p.prefix_chunks;
+  s.own_chunks = (int)p.own_chunks;
+  s.prefix_tiles = (int)p.prefix_tiles;
+  s.own_tiles = p.own_tiles;
+  s.prefix_units = (int)p.prefix_units;
   s.slots = (int)(p.prefix_chunks + p.own_chunks);
   const size_t parts = (size_t)a->B * a->s_tkg * a->nq * s.slots;
   Carver c{static_cast<char*>(workspace), workspace_bytes};

@@ -566,14 +566,16 @@ hipError_t moe_finalize_launch(const float* ybuf, int T, int K, int H, const int
 hipError_t kv_append_launch(const mkd_kv_append_args& a, hipStream_t s);
 // attn_shared.hip: how a call's positions split into blocks, from its shapes alone
 struct SharedPlan {
-  int prefix_qt, own_qt, own_tiles;       // 16-row tiles per block; tiles of one sequence's rows
-  long long prefix_tiles;                 // row tiles of all groups, at most
-  int prefix_chunk, own_chunk;            // positions per block
-  long long prefix_chunks, own_chunks;
+  int prefix_qt, own_qt;                  // 16-row tiles per wave of staged prefixes (0: direct), of direct units
+  int own_tiles;                          // tiles of one sequence's rows
+  long long prefix_tiles;                 // tiles of all groups' rows, at most
+  int prefix_chunk, own_chunk;            // positions per unit
+  long long prefix_chunks, own_chunks, prefix_units, own_units;
 };
 struct SharedArgs {
   mkd_shared_prefix_args p;
-  int prefix_chunk, own_chunk, prefix_chunks, slots;   // slots: partials per row
+  int prefix_chunk, own_chunk, prefix_chunks, own_chunks, prefix_tiles, own_tiles, prefix_units;
+  int slots;                              // partials per row
   float *part_o, *part_ml;                // [rows][slots][d], [rows][slots][2]
 };
 SharedPlan shared_plan(const mkd_shared_prefix_args& p);
