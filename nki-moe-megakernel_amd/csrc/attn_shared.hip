@@ -24,8 +24,8 @@
 // positions): the waves take steps of their own, rows straight to registers a step ahead,
 // and merge at the end: nothing to share, and no barrier to wait at.
 //
-// The rows' addresses are formed once per chunk in LDS, so blocks of any length may end
-// inside a tile; a position past the length or in no valid block reads a row of zeros
+// The rows' places in the caches are formed once per chunk in LDS, so blocks of any length
+// may end inside a tile; a position past the length or in no valid block is a row of zeros
 // (so that what a page holds behind a sequence, NaN among it, never meets a product).
 #include "common.h"
 #include "mkd_internal.h"
@@ -118,24 +118,25 @@ MKD_DEV void load_q(const SharedArgs& a, const Unit& u, int first, u32x4_t (&qf)
     lim[t] = u.own ? u.len - (S - 1 - s) : u.len;
   }
 }
-// Byte offsets of the chunk's rows in the caches, -1: a row of zeros.
-MKD_DEV void fill_offsets(const SharedArgs& a, const Unit& u, int eb, int n, long long* koff, long long* voff) {
+// Places of the chunk's rows in the caches, in units of 16 bytes; kNoRow: a row of zeros.
+constexpr uint32_t kNoRow = 0xffffffffu;
+MKD_DEV void fill_places(const SharedArgs& a, const Unit& u, int eb, int n, uint32_t* kat, uint32_t* vat) {
   for (int i = threadIdx.x; i < n; i += 64 * kShWaves) {
     const int t = u.chunk0 + i;
-    long long k = -1, v = -1;
+    uint32_t k = kNoRow, v = kNoRow;
     if (t < u.len) {
       const int blk = u.table[t / a.p.block_len], r = t % a.p.block_len;
       if ((unsigned)blk < (unsigned)a.p.num_blocks) {
-        k = (blk * a.p.k_cache_stride[0] + r * a.p.k_cache_stride[1] + u.kvh * a.p.k_cache_stride[2]) * eb;
-        v = (blk * a.p.v_cache_stride[0] + r * a.p.v_cache_stride[1] + u.kvh * a.p.v_cache_stride[2]) * eb;
+        k = (uint32_t)((blk * a.p.k_cache_stride[0] + r * a.p.k_cache_stride[1] + u.kvh * a.p.k_cache_stride[2]) * eb / 16);
+        v = (uint32_t)((blk * a.p.v_cache_stride[0] + r * a.p.v_cache_stride[1] + u.kvh * a.p.v_cache_stride[2]) * eb / 16);
       }
     }
-    koff[i] = k;
-    voff[i] = v;
+    kat[i] = k;
+    vat[i] = v;
   }
 }
-MKD_DEV gptr row_at(const void* cache, long long off) {
-  return (gptr)(off < 0 ? reinterpret_cast<const char*>(g_zero_row) : static_cast<const char*>(cache) + off);
+MKD_DEV gptr row_at(const void* cache, uint32_t at) {
+  return (gptr)(at == kNoRow ? reinterpret_cast<const char*>(g_zero_row) : static_cast<const char*>(cache) + at * 16ull);
 }
 
 // The running softmax of one wave's rows: scores of a step to probabilities, and what
@@ -212,8 +213,8 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
   constexpr int NK = D / 32, NDT = D / 16, ROWS = 16 * QT;
   constexpr int KL = D * EB / 64;               // 16-byte loads of a lane's K row share
   constexpr int VD = D * EB / 64;               // dwords of a lane's V row share
-  long long* const koff = reinterpret_cast<long long*>(mem);
-  long long* const voff = koff + kShMaxChunk;
+  uint32_t* const kat = reinterpret_cast<uint32_t*>(mem);
+  uint32_t* const vat = kat + kShMaxChunk;
   float* const o_s = reinterpret_cast<float*>(mem);
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -222,7 +223,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
   u32x4_t qf[QT][NK];
   int lim[QT];
   load_q<D, QT, FP8>(a, un, 0, qf, lim);
-  fill_offsets(a, un, EB, nst * kShStep, koff, voff);
+  fill_places(a, un, EB, nst * kShStep, kat, vat);
   const int lim_min = un.own ? un.len - (a.p.s_tkg - 1) : un.len;
   const float scale2 = scale_log2(a);
   __syncthreads();
@@ -232,7 +233,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
   auto load_k = [&](int st) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const gptr p = row_at(a.p.k_cache, koff[st * kShStep + 16 * u + col]);
+      const gptr p = row_at(a.p.k_cache, kat[st * kShStep + 16 * u + col]);
 #pragma unroll
       for (int j = 0; j < KL; ++j) kr[u][j] = g_ld16(p + (FP8 ? q4 * (D / 4) + 16 * j : q4 * 16 + 64 * j));
     }
@@ -242,7 +243,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const gptr p = row_at(a.p.v_cache, voff[st * kShStep + 16 * u + 4 * q4 + j]) + col * (4 * VD);
+        const gptr p = row_at(a.p.v_cache, vat[st * kShStep + 16 * u + 4 * q4 + j]) + col * (4 * VD);
         if constexpr (VD == 4) {
           const u32x4_t v = g_ld16(p);
 #pragma unroll
@@ -317,7 +318,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
     if (sn < nst) load_v(sn);
   }
   // ---- merge the waves into this chunk's partial ----
-  __syncthreads();                              // the offsets are read; o_s takes their place
+  __syncthreads();                              // the places are read; o_s takes theirs
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     if (lane < 16) m_s[w][16 * t + lane] = rows.m[t];
@@ -356,12 +357,24 @@ MKD_DEV void g_to_lds16(gptr src, char* dst) {   // lane l's 16 bytes to dst + 1
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                    (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
-// Four 16-bit values of one column: per 16 lanes a tile of 4 rows x 16, lane i naming the
-// 8 bytes of row i / 4 and columns 4 (i % 4) .., lane j getting column j.
-typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
-MKD_DEV uint2 lds_tr8(const char* p) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p));
+// V operands of 4 d-tiles: out[2 i + u] from at[i] and OFF * u bytes behind it.  Per 16 lanes
+// the instruction takes a tile of 4 rows x 16 of 16-bit values, lane i naming the 8 bytes of
+// row i / 4 and columns 4 (i % 4) .., and gives lane j column j.  (Written out, with its wait:
+// after the builtin's form the compiler waits for every copy to LDS in flight.)
+template <int OFF>
+MKD_DEV void lds_tr8(uint64_t (&out)[8], const uint32_t (&at)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(out[0]), "=&v"(out[1]), "=&v"(out[2]), "=&v"(out[3]), "=&v"(out[4]), "=&v"(out[5]), "=&v"(out[6]),
+        "=&v"(out[7])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFF)
+      : "memory");
 }
+MKD_DEV uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
 template <int N>
 MKD_DEV void wait_loads() {                     // all but the last N vector memory accesses
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
@@ -378,8 +391,8 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
   constexpr int kStage = 2 * kShStep * RB, CPW = CPR / kShWaves;   // 1 KiB copies per wave and stage
   static_assert(CPW >= 1, "a copy per wave");
   char* const ring = mem;
-  long long* const koff = reinterpret_cast<long long*>(mem + kShStages * kStage);
-  long long* const voff = koff + kShMaxChunk;
+  uint32_t* const kat = reinterpret_cast<uint32_t*>(mem + kShStages * kStage);
+  uint32_t* const vat = kat + kShMaxChunk;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q4 = lane >> 4, col = lane & 15;
@@ -388,36 +401,38 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
   u32x4_t qf[QT][NK];
   int lim[QT];
   load_q<D, QT, FP8>(a, un, first, qf, lim);
-  fill_offsets(a, un, EB, nst * kShStep, koff, voff);
+  fill_places(a, un, EB, nst * kShStep, kat, vat);
   const float scale2 = scale_log2(a);
   __syncthreads();
-  auto copy = [&](int st) {
-    char* const dst = ring + (st % kShStages) * kStage;
+  // (the stage read, the stage filled and the places never overlap: without that promise the
+  // compiler waits for the copies in flight in front of every read)
+  auto copy = [&](char* __restrict dst, const uint32_t* __restrict ka, const uint32_t* __restrict va) {
+    uint32_t at[CPW];
 #pragma unroll
     for (int i = 0; i < CPW; ++i) {
       const int n = w * CPW + i;                // (uniform) the stage's n-th KiB: K in the first half
+      at[i] = n >= CPR / 2 ? va[((n - CPR / 2) * 64 + lane) / CPR] : ka[(n * 64 + lane) / CPR];
+    }
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) {
+      const int n = w * CPW + i;
       const bool v = n >= CPR / 2;
       const int piece = (v ? n - CPR / 2 : n) * 64 + lane, row = piece / CPR, p = piece % CPR;
-      const gptr src = row_at(v ? a.p.v_cache : a.p.k_cache, (v ? voff : koff)[st * kShStep + row]);
-      g_to_lds16(src + ((p ^ (row & (CPR - 1))) << 4), dst + n * 1024);
+      g_to_lds16(row_at(v ? a.p.v_cache : a.p.k_cache, at[i]) + ((p ^ (row & (CPR - 1))) << 4), dst + n * 1024);
     }
   };
-  copy(0);
-  if (nst > 1) copy(1);
+#pragma unroll 1
+  for (int st = 0; st < min(nst, 2); ++st) copy(ring + st * kStage, kat + st * kShStep, vat + st * kShStep);
   Rows<QT, NDT> rows;
   const bool live = first < un.nrow;            // (uniform)
   // operand reads: K row 16 u + col, V rows 16 u + 4 q4 + ..
   const int kx = (col & (CPR - 1)) << 4;
   const int vrow = 4 * q4 + (col >> 2), vx = (vrow & (CPR - 1)) << 4;
-  for (int st = 0; st < nst; ++st) {
-    if (st + 1 < nst) wait_loads<CPW>();        // stage st landed: this wave's part ..
-    else wait_loads<0>();
-    lds_barrier();                              // .. and everyone's; stage st - 1 is read
-    if (st + 2 < nst) copy(st + 2);
-    if (!live) continue;
-    const char* const ks = ring + (st % kShStages) * kStage;
+  auto step = [&](const char* __restrict ks, char* __restrict dst, const uint32_t* __restrict ka,
+                  const uint32_t* __restrict va, int p0, bool more) {
+    if (more) copy(dst, ka, va);
+    if (!live) return;
     const char* const vs = ks + kShStep * RB;
-    const int p0 = un.chunk0 + st * kShStep;
     f32x4_t sc[QT][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -477,22 +492,33 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
       }
     } else {
       // d-tile dt is the elements 16 dt + col, transposed by the read itself
+      const uint32_t base = lds_address(vs) + vrow * RB + (col & 1) * 8;
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) {
-        u32x4_t bop;
+      for (int d0 = 0; d0 < NDT; d0 += 4) {
+        uint32_t at[4];
+        uint64_t v[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint2 v = lds_tr8(vs + (16 * u + vrow) * RB + (((2 * dt + ((col >> 1) & 1)) << 4) ^ vx) + (col & 1) * 8);
-          bop[2 * u] = v.x;
-          bop[2 * u + 1] = v.y;
+        for (int i = 0; i < 4; ++i) at[i] = base + (((2 * (d0 + i) + ((col >> 1) & 1)) << 4) ^ vx);
+        lds_tr8<16 * RB>(v, at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const u32x4_t bop = {(uint32_t)v[2 * i], (uint32_t)(v[2 * i] >> 32), (uint32_t)v[2 * i + 1],
+                               (uint32_t)(v[2 * i + 1] >> 32)};
+#pragma unroll
+          for (int t = 0; t < QT; ++t) rows.o[t][d0 + i] = mfma16x16x32(ph[t], bop, rows.o[t][d0 + i]);
         }
-#pragma unroll
-        for (int t = 0; t < QT; ++t) rows.o[t][dt] = mfma16x16x32(ph[t], bop, rows.o[t][dt]);
       }
     }
+  };
+  for (int st = 0; st < nst; ++st) {
+    if (st + 1 < nst) wait_loads<CPW>();        // stage st landed: this wave's part ..
+    else wait_loads<0>();
+    lds_barrier();                              // .. and everyone's; stage st - 1 is read
+    step(ring + st % kShStages * kStage, ring + (st + 2) % kShStages * kStage, kat + (st + 2) * kShStep,
+         vat + (st + 2) * kShStep, un.chunk0 + st * kShStep, st + 2 < nst);
   }
   // ---- the wave's rows out, through LDS in the order of the head's elements ----
-  __syncthreads();                              // every stage and offset is read
+  __syncthreads();                              // every stage and place is read
   if (!live) return;
   float* const o_s = reinterpret_cast<float*>(mem) + w * 16 * D;   // 16 rows at a time
   const int n = min(un.nrow - first, 16 * QT);
@@ -530,7 +556,7 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
 // direct units.
 template <int D, bool FP8, int PQ, int OQ>
 __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArgs a) {
-  constexpr int EB = FP8 ? 1 : 2, kTab = 2 * kShMaxChunk * 8;
+  constexpr int EB = FP8 ? 1 : 2, kTab = 2 * kShMaxChunk * 4;
   constexpr int kDirect = kShWaves * 16 * OQ * D * 4 > kTab ? kShWaves * 16 * OQ * D * 4 : kTab;
   constexpr int kStaged = PQ > 0 ? kShStages * 2 * kShStep * D * EB + kTab : 0;
   constexpr int kMem = kDirect > kStaged ? kDirect : kStaged;
@@ -613,22 +639,33 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
   for (int i = lane; i < n; i += 64) M = fmaxf(M, ml[2 * slot_of(i)]);
   M = wave_max(M);
   const float ms = M == -INFINITY ? 0.f : M;
-  float L = a.p.sink ? exp2_hw(a.p.sink[h] * kLog2e - ms) : 0.f;
-  float o[D / 64];
-#pragma unroll
-  for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
+  // 16 bytes of a partial per lane: the wave takes 64 / (D / 4) partials at a time
+  constexpr int LP = D / 4, PW = 64 / LP;
+  const int sub = lane / LP, d = lane % LP * 4;
+  float L = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
+  for (int i = sub; i < n; i += PW) {
     const int c = slot_of(i);
-    const float f = exp2_hw(ml[2 * c] - ms);     // (a chunk that the row does not see: 0)
-    L += ml[2 * c + 1] * f;
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] += po[(long long)c * D + lane * (D / 64) + e] * f;
+    const float2 x = *reinterpret_cast<const float2*>(ml + 2 * c);
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(po + (long long)c * D + d);
+    const float f = exp2_hw(x.x - ms);           // (a chunk that the row does not see: 0)
+    L += x.y * f;
+    o += v * f;
   }
+#pragma unroll
+  for (int k = LP; k < 64; k <<= 1) {
+    L += __shfl_xor(L, k, 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], k, 64);
+  }
+  if (a.p.sink) L += exp2_hw(a.p.sink[h] * kLog2e - ms);
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
   uint16_t* dst = static_cast<uint16_t*>(a.p.out) + b * a.p.out_stride[0] + s * a.p.out_stride[1] + h * a.p.out_stride[2];
-  if constexpr (D == 128) *reinterpret_cast<uint32_t*>(dst + 2 * lane) = pack2bf(o[0] * inv, o[1] * inv);
-  else dst[lane] = (uint16_t)f2bf(o[0] * inv);
+  if (sub == 0) {
+    reinterpret_cast<uint32_t*>(dst + d)[0] = pack2bf(o[0] * inv, o[1] * inv);
+    reinterpret_cast<uint32_t*>(dst + d)[1] = pack2bf(o[2] * inv, o[3] * inv);
+  }
 }
 
 // Shapes alone decide the split (lengths stay on the device).

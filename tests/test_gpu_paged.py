@@ -277,11 +277,15 @@ def test_offsets_past_32_bits(mk, dev):
     mk.kv_append_rope(q, k, v, None, None, None, K, V, slots)
     assert torch.equal(K[last, :T], k) and torch.equal(V[last, :T], v)
     i32 = dict(dtype=torch.int32, device=dev)
-    got = mk.attention_shared_prefix(q[:1], K, V, None, None, None, torch.tensor([[last]], **i32), torch.tensor([T], **i32))
     kc, vc = k.cpu()[None], v.cpu()[None]
-    want = O.attention_shared_prefix(q[:1, None].cpu(), kc, vc, None, None, None, torch.zeros(1, 1, dtype=torch.int32),
-                                     torch.tensor([T]), d ** -0.5)
-    check_attention(got, want)
+    # a sequence's own rows, and a prefix of 40 sequences (80 query rows a kv head)
+    own = mk.attention_shared_prefix(q[:1], K, V, None, None, None, torch.tensor([[last]], **i32), torch.tensor([T], **i32))
+    shared = mk.attention_shared_prefix(q, K, V, torch.tensor([[last]], **i32), torch.tensor([T], **i32),
+                                        torch.tensor([0, T], **i32), torch.zeros(T, 0, **i32), torch.zeros(T, **i32))
+    want = O.attention_shared_prefix(q[:, None].cpu(), kc, vc, torch.zeros(1, 1, dtype=torch.int32), torch.tensor([T]),
+                                     torch.tensor([0, T]), torch.zeros(T, 0), torch.zeros(T), d ** -0.5)
+    check_attention(own, [w[:1] for w in want])
+    check_attention(shared, want)
 
 
 def test_streams_and_graph(mk, dev):
