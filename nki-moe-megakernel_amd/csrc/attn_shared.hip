@@ -91,7 +91,6 @@ constexpr int kShStages = 3;                    // LDS ring of the staged form
 // One unit: `nrow` query rows (from row0 of the sequences from b0 on) against the
 // positions [chunk0, min(chunk0 + CP, len)) of one table, as partial `slot`.
 struct Unit {
-  const int* table;
   int b0, row0, nrow, len, chunk0, CP, kvh, slot, width;
   bool own;                                     // new token i sees len - (S - 1 - i) positions
 };
@@ -118,25 +117,44 @@ MKD_DEV void load_q(const SharedArgs& a, const Unit& u, int first, u32x4_t (&qf)
     lim[t] = u.own ? u.len - (S - 1 - s) : u.len;
   }
 }
-// Places of the chunk's rows in the caches, in units of 16 bytes; kNoRow: a row of zeros.
-constexpr uint32_t kNoRow = 0xffffffffu;
-MKD_DEV void fill_places(const SharedArgs& a, const Unit& u, int eb, int n, uint32_t* kat, uint32_t* vat) {
-  for (int i = threadIdx.x; i < n; i += 64 * kShWaves) {
-    const int t = u.chunk0 + i;
-    uint32_t k = kNoRow, v = kNoRow;
-    if (t < u.len) {
-      const int blk = u.table[t / a.p.block_len], r = t % a.p.block_len;
-      if ((unsigned)blk < (unsigned)a.p.num_blocks) {
-        k = (uint32_t)((blk * a.p.k_cache_stride[0] + r * a.p.k_cache_stride[1] + u.kvh * a.p.k_cache_stride[2]) * eb / 16);
-        v = (uint32_t)((blk * a.p.v_cache_stride[0] + r * a.p.v_cache_stride[1] + u.kvh * a.p.v_cache_stride[2]) * eb / 16);
-      }
+// Addresses of the chunk's rows in the caches; a row of zeros for a position past the
+// length or in no valid block.  The table is read before the length is known.
+struct Places {
+  int blk[kShMaxChunk / (64 * kShWaves)];
+  MKD_DEV void load(const SharedArgs& a, const int* table, int width, int chunk0, int CP) {
+#pragma unroll
+    for (int k = 0; k < kShMaxChunk / (64 * kShWaves); ++k) {
+      const int i = threadIdx.x + 64 * kShWaves * k;
+      blk[k] = i < CP ? table[min((chunk0 + i) / a.p.block_len, width - 1)] : -1;
     }
-    kat[i] = k;
-    vat[i] = v;
   }
-}
-MKD_DEV gptr row_at(const void* cache, uint32_t at) {
-  return (gptr)(at == kNoRow ? reinterpret_cast<const char*>(g_zero_row) : static_cast<const char*>(cache) + at * 16ull);
+  MKD_DEV void store(const SharedArgs& a, const Unit& u, int eb, int n, uint64_t* kat, uint64_t* vat) const {
+    const char* const kc = static_cast<const char*>(a.p.k_cache) + u.kvh * a.p.k_cache_stride[2] * eb;
+    const char* const vc = static_cast<const char*>(a.p.v_cache) + u.kvh * a.p.v_cache_stride[2] * eb;
+#pragma unroll
+    for (int k = 0; k < kShMaxChunk / (64 * kShWaves); ++k) {
+      const int i = threadIdx.x + 64 * kShWaves * k, t = u.chunk0 + i;
+      if (i >= n) break;
+      const char *ka = reinterpret_cast<const char*>(g_zero_row), *va = ka;
+      if (t < u.len && (unsigned)blk[k] < (unsigned)a.p.num_blocks) {
+        const int r = t % a.p.block_len;
+        ka = kc + (blk[k] * a.p.k_cache_stride[0] + r * a.p.k_cache_stride[1]) * eb;
+        va = vc + (blk[k] * a.p.v_cache_stride[0] + r * a.p.v_cache_stride[1]) * eb;
+      }
+      kat[i] = reinterpret_cast<uint64_t>(ka);
+      vat[i] = reinterpret_cast<uint64_t>(va);
+    }
+  }
+};
+
+// (a NaN wins; without the canonicalisation that fmaxf's operands get)
+MKD_DEV float most(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+// the largest over the four lanes sharing lane % 16
+MKD_DEV float quad_rows_max(float x) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = most(__uint_as_float(h[0]), __uint_as_float(h[1]));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return most(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // The running softmax of one wave's rows: scores of a step to probabilities, and what
@@ -154,16 +172,16 @@ struct Rows {
       for (int dt = 0; dt < NDT; ++dt) o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
   }
-  // raw products sc of tile t (times scale2: scores); its P operand
+  // Raw products sc of tile t (times scale2: scores) to its P operand.  The maximum that the
+  // exponentials refer to follows the largest score only where that is more than 2^8 above
+  // it: the sums keep their relative precision, and the accumulators are seldom rescaled.
   MKD_DEV u32x4_t weigh(int t, const f32x4_t (&sc)[2], float scale2) {
     const int q4 = (threadIdx.x & 63) >> 4;
-    float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
-    mx = fmaxf(mx, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
-    const float mn = fmaxf(m[t], mx);
-    if (__any(mn > m[t])) {                     // uniform: a maximum moved
-      const float alpha = m[t] == -INFINITY ? 0.f : exp2_hw(m[t] - mn);
+    float mx = most(most(sc[0][0], sc[0][1]), sc[0][2]);
+    mx = most(most(mx, sc[0][3]), sc[1][0]);
+    mx = quad_rows_max(most(most(most(mx, sc[1][1]), sc[1][2]), sc[1][3])) * scale2;
+    if (__any(mx > m[t] + 8.f)) {               // uniform
+      const float mn = most(m[t], mx), alpha = m[t] == -INFINITY ? 0.f : exp2_hw(m[t] - mn);
       m[t] = mn;
       float al[4];                              // (o and l rows are 4 q4 + i)
 #pragma unroll
@@ -175,13 +193,13 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[t][dt][i] *= al[i];
     }
-    const float ms = m[t] == -INFINITY ? 0.f : m[t];
+    const float ms = m[t] == -INFINITY ? 0.f : -m[t];
     u32x4_t ph;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = exp2_hw(fmaf(sc[u][i], scale2, -ms));
+      for (int i = 0; i < 4; ++i) p[i] = exp2_hw(fmaf(sc[u][i], scale2, ms));
       ph[2 * u] = pack2bf(p[0], p[1]);
       ph[2 * u + 1] = pack2bf(p[2], p[3]);
     }
@@ -206,15 +224,21 @@ MKD_DEV long long part_at(const SharedArgs& a, const Unit& u, int r) {   // the 
   return (((long long)(u.b0 + rr / r1) * S + (rr / gqa) % S) * a.p.nq + u.kvh * gqa + rr % gqa) * a.slots + u.slot;
 }
 
+// A partial's elements lie as a lane holds them: bf16 caches' at (d % 16) D / 16 + d / 16
+// (the transposed reads give lane column d % 16 the elements 16 apart), e4m3's at d.
+template <int D, bool FP8>
+MKD_DEV int element_of(int at) { return FP8 ? at : at % (D / 16) * 16 + at / (D / 16); }
+
 // ---- direct: position steps w, w + 4, .. to wave w, the waves merged at the end ----
 template <int D, int QT, bool FP8>
-MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (*m_s)[32], float (*l_s)[32]) {
+MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& places, char* mem, float (*m_s)[32],
+                         float (*l_s)[32]) {
   constexpr int EB = FP8 ? 1 : 2;               // bytes per cached element
   constexpr int NK = D / 32, NDT = D / 16, ROWS = 16 * QT;
   constexpr int KL = D * EB / 64;               // 16-byte loads of a lane's K row share
   constexpr int VD = D * EB / 64;               // dwords of a lane's V row share
-  uint32_t* const kat = reinterpret_cast<uint32_t*>(mem);
-  uint32_t* const vat = kat + kShMaxChunk;
+  uint64_t* const kat = reinterpret_cast<uint64_t*>(mem);
+  uint64_t* const vat = kat + kShMaxChunk;
   float* const o_s = reinterpret_cast<float*>(mem);
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -223,7 +247,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
   u32x4_t qf[QT][NK];
   int lim[QT];
   load_q<D, QT, FP8>(a, un, 0, qf, lim);
-  fill_places(a, un, EB, nst * kShStep, kat, vat);
+  places.store(a, un, EB, nst * kShStep, kat, vat);
   const int lim_min = un.own ? un.len - (a.p.s_tkg - 1) : un.len;
   const float scale2 = scale_log2(a);
   __syncthreads();
@@ -233,7 +257,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
   auto load_k = [&](int st) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const gptr p = row_at(a.p.k_cache, kat[st * kShStep + 16 * u + col]);
+      const gptr p = (gptr)kat[st * kShStep + 16 * u + col];
 #pragma unroll
       for (int j = 0; j < KL; ++j) kr[u][j] = g_ld16(p + (FP8 ? q4 * (D / 4) + 16 * j : q4 * 16 + 64 * j));
     }
@@ -243,7 +267,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const gptr p = row_at(a.p.v_cache, vat[st * kShStep + 16 * u + 4 * q4 + j]) + col * (4 * VD);
+        const gptr p = (gptr)vat[st * kShStep + 16 * u + 4 * q4 + j] + col * (4 * VD);
         if constexpr (VD == 4) {
           const u32x4_t v = g_ld16(p);
 #pragma unroll
@@ -318,7 +342,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
     if (sn < nst) load_v(sn);
   }
   // ---- merge the waves into this chunk's partial ----
-  __syncthreads();                              // the places are read; o_s takes theirs
+  __syncthreads();                              // the addresses are read; o_s takes their place
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     if (lane < 16) m_s[w][16 * t + lane] = rows.m[t];
@@ -334,7 +358,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
   }
   __syncthreads();
   for (int idx = threadIdx.x * 4; idx < un.nrow * D; idx += 64 * kShWaves * 4) {
-    const int r = idx / D, d = idx % D;
+    const int r = idx / D, e0 = idx % D;
     float M = -INFINITY;
 #pragma unroll
     for (int q = 0; q < kShWaves; ++q) M = fmaxf(M, m_s[q][r]);
@@ -344,11 +368,12 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, char* mem, float (
     for (int q = 0; q < kShWaves; ++q) {
       const float f = m_s[q][r] == -INFINITY ? 0.f : exp2_hw(m_s[q][r] - M);
       L += l_s[q][r] * f;
-      O += *reinterpret_cast<const f32x4_t*>(o_s + ((q * ROWS + r) * D + d)) * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] += o_s[(q * ROWS + r) * D + element_of<D, FP8>(e0 + e)] * f;
     }
     const long long at = part_at(a, un, r);
-    *reinterpret_cast<f32x4_t*>(a.part_o + at * D + d) = O;
-    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{M, L};
+    *reinterpret_cast<f32x4_t*>(a.part_o + at * D + e0) = O;
+    if (e0 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{M, L};
   }
 }
 
@@ -385,14 +410,14 @@ MKD_DEV void wait_loads() {                     // all but the last N vector mem
 // row's piece p ^ r (modulo the pieces of a row), so that the 16 rows of an operand read
 // lie on different banks.
 template <int D, int QT, bool FP8>
-MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
+MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& places, char* mem) {
   constexpr int EB = FP8 ? 1 : 2, NK = D / 32, NDT = D / 16;
   constexpr int RB = D * EB, CPR = RB / 16;     // bytes, pieces of a row
   constexpr int kStage = 2 * kShStep * RB, CPW = CPR / kShWaves;   // 1 KiB copies per wave and stage
   static_assert(CPW >= 1, "a copy per wave");
   char* const ring = mem;
-  uint32_t* const kat = reinterpret_cast<uint32_t*>(mem + kShStages * kStage);
-  uint32_t* const vat = kat + kShMaxChunk;
+  uint64_t* const kat = reinterpret_cast<uint64_t*>(mem + kShStages * kStage);
+  uint64_t* const vat = kat + kShMaxChunk;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q4 = lane >> 4, col = lane & 15;
@@ -401,13 +426,13 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
   u32x4_t qf[QT][NK];
   int lim[QT];
   load_q<D, QT, FP8>(a, un, first, qf, lim);
-  fill_places(a, un, EB, nst * kShStep, kat, vat);
+  places.store(a, un, EB, nst * kShStep, kat, vat);
   const float scale2 = scale_log2(a);
   __syncthreads();
-  // (the stage read, the stage filled and the places never overlap: without that promise the
+  // (the stage read, the stage filled and the addresses never overlap: without that promise the
   // compiler waits for the copies in flight in front of every read)
-  auto copy = [&](char* __restrict dst, const uint32_t* __restrict ka, const uint32_t* __restrict va) {
-    uint32_t at[CPW];
+  auto copy = [&](char* __restrict dst, const uint64_t* __restrict ka, const uint64_t* __restrict va) {
+    uint64_t at[CPW];
 #pragma unroll
     for (int i = 0; i < CPW; ++i) {
       const int n = w * CPW + i;                // (uniform) the stage's n-th KiB: K in the first half
@@ -416,9 +441,8 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
 #pragma unroll
     for (int i = 0; i < CPW; ++i) {
       const int n = w * CPW + i;
-      const bool v = n >= CPR / 2;
-      const int piece = (v ? n - CPR / 2 : n) * 64 + lane, row = piece / CPR, p = piece % CPR;
-      g_to_lds16(row_at(v ? a.p.v_cache : a.p.k_cache, at[i]) + ((p ^ (row & (CPR - 1))) << 4), dst + n * 1024);
+      const int piece = (n >= CPR / 2 ? n - CPR / 2 : n) * 64 + lane, row = piece / CPR, p = piece % CPR;
+      g_to_lds16((gptr)at[i] + ((p ^ (row & (CPR - 1))) << 4), dst + n * 1024);
     }
   };
 #pragma unroll 1
@@ -428,8 +452,8 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
   // operand reads: K row 16 u + col, V rows 16 u + 4 q4 + ..
   const int kx = (col & (CPR - 1)) << 4;
   const int vrow = 4 * q4 + (col >> 2), vx = (vrow & (CPR - 1)) << 4;
-  auto step = [&](const char* __restrict ks, char* __restrict dst, const uint32_t* __restrict ka,
-                  const uint32_t* __restrict va, int p0, bool more) {
+  auto step = [&](const char* __restrict ks, char* __restrict dst, const uint64_t* __restrict ka,
+                  const uint64_t* __restrict va, int p0, bool more) {
     if (more) copy(dst, ka, va);
     if (!live) return;
     const char* const vs = ks + kShStep * RB;
@@ -517,37 +541,25 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
     step(ring + st % kShStages * kStage, ring + (st + 2) % kShStages * kStage, kat + (st + 2) * kShStep,
          vat + (st + 2) * kShStep, un.chunk0 + st * kShStep, st + 2 < nst);
   }
-  // ---- the wave's rows out, through LDS in the order of the head's elements ----
-  __syncthreads();                              // every stage and place is read
   if (!live) return;
-  float* const o_s = reinterpret_cast<float*>(mem) + w * 16 * D;   // 16 rows at a time
+  // ---- the wave's rows out: row 4 q4 + i of tile t, its sum from every lane column, its
+  // maximum from lane column 4 q4 + i (a lane forms one row's place, the others ask it) ----
   const int n = min(un.nrow - first, 16 * QT);
+  const long long place = part_at(a, un, first + min(lane % (16 * QT), n - 1));
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
+  for (int t = 0; t < QT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * t + 4 * q4 + i;
+      const long long at = __shfl(place, r, 64);
+      const float mx = __shfl(rows.m[t], 4 * q4 + i, 64);
+      if (r >= n) continue;
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) o_s[(4 * q4 + i) * D + (FP8 ? col * NDT + dt : 16 * dt + col)] = rows.o[t][dt][i];
-    wave_lds_sync();
-    for (int idx = lane * 4; idx < 16 * D; idx += 256) {
-      const int r = 16 * t + idx / D;
-      if (r < n)
-        *reinterpret_cast<f32x4_t*>(a.part_o + part_at(a, un, first + r) * D + idx % D) =
-            *reinterpret_cast<const f32x4_t*>(o_s + idx);
+      for (int q = 0; q < NDT / 4; ++q)
+        *reinterpret_cast<f32x4_t*>(a.part_o + at * D + col * NDT + 4 * q) =
+            f32x4_t{rows.o[t][4 * q][i], rows.o[t][4 * q + 1][i], rows.o[t][4 * q + 2][i], rows.o[t][4 * q + 3][i]};
+      if (col == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{mx, rows.l[t][i]};
     }
-    wave_lds_sync();
-    // row 4 q4 + i: its sum from lane column 0, its maximum from lane column 4 q4 + i
-    float mx[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mx[i] = __shfl(rows.m[t], 4 * q4 + i, 64);
-    if (col == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * t + 4 * q4 + i;
-        if (r < n) *reinterpret_cast<float2*>(a.part_ml + part_at(a, un, first + r) * 2) = float2{mx[i], rows.l[t][i]};
-      }
-    }
-  }
 }
 
 }  // namespace
@@ -556,16 +568,16 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, char* mem) {
 // direct units.
 template <int D, bool FP8, int PQ, int OQ>
 __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArgs a) {
-  constexpr int EB = FP8 ? 1 : 2, kTab = 2 * kShMaxChunk * 4;
+  constexpr int EB = FP8 ? 1 : 2, kTab = 2 * kShMaxChunk * 8;
   constexpr int kDirect = kShWaves * 16 * OQ * D * 4 > kTab ? kShWaves * 16 * OQ * D * 4 : kTab;
   constexpr int kStaged = PQ > 0 ? kShStages * 2 * kShStep * D * EB + kTab : 0;
   constexpr int kMem = kDirect > kStaged ? kDirect : kStaged;
-  static_assert(kMem >= kShWaves * 16 * D * 4, "a wave's 16 rows out");
   __shared__ __attribute__((aligned(1024))) char mem[kMem];
   __shared__ float m_s[kShWaves][32], l_s[kShWaves][32];
   const int r1 = a.p.s_tkg * (a.p.nq / a.p.nkv);
   int L = blockIdx.x;
   Unit u;
+  Places places;
   if (L < a.prefix_units) {
     // the tiles of one (chunk, kv head) on one XCD (workgroups go round-robin by index)
     constexpr int per = PQ > 0 ? kShWaves * 16 * PQ : 16 * OQ;
@@ -573,18 +585,25 @@ __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArg
     const int c = cell / a.p.nkv;
     if (c >= a.prefix_chunks) return;
     int g, first;
-    if (!find_tile(a, tile, per, r1, threadIdx.x & 63, g, first)) return;
+    u.width = a.p.prefix_blocks;
+    u.CP = a.prefix_chunk;
+    u.chunk0 = c * u.CP;
+    if (a.p.G == 1) {                           // (its table at once)
+      g = 0;
+      first = tile;
+      places.load(a, a.p.prefix_tables, u.width, u.chunk0, u.CP);
+    } else {
+      if (!find_tile(a, tile, per, r1, threadIdx.x & 63, g, first)) return;
+      places.load(a, a.p.prefix_tables + (long long)g * u.width, u.width, u.chunk0, u.CP);
+    }
     const int lo = min(max(a.p.prefix_starts[g], 0), a.p.B), hi = min(max(a.p.prefix_starts[g + 1], lo), a.p.B);
     u.own = false;
     u.b0 = lo;
     u.row0 = first * per;
     u.nrow = min((hi - lo) * r1 - u.row0, per);
-    u.width = a.p.prefix_blocks;
-    u.table = a.p.prefix_tables + (long long)g * u.width;
     u.len = a.p.prefix_lens[g];
     u.kvh = cell % a.p.nkv;
     u.slot = c;
-    u.CP = a.prefix_chunk;
   } else {
     L -= a.prefix_units;
     const int c = L % a.own_chunks, rest = L / a.own_chunks, tile = rest / a.p.nkv % a.own_tiles;
@@ -594,28 +613,28 @@ __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArg
     u.row0 = tile * 16 * OQ;
     u.nrow = min(r1 - u.row0, 16 * OQ);
     u.width = a.p.own_blocks;
-    u.table = a.p.tables + (long long)u.b0 * u.width;
+    u.CP = a.own_chunk;
+    u.chunk0 = c * u.CP;
+    places.load(a, a.p.tables + (long long)u.b0 * u.width, u.width, u.chunk0, u.CP);
     u.len = a.p.lens[u.b0];
     u.slot = a.prefix_chunks + c;
-    u.CP = a.own_chunk;
   }
-  u.chunk0 = (u.own ? u.slot - a.prefix_chunks : u.slot) * u.CP;
   u.len = __builtin_amdgcn_readfirstlane(min(max(u.len, 0), u.width * a.p.block_len));
   u.b0 = __builtin_amdgcn_readfirstlane(u.b0);
   u.row0 = __builtin_amdgcn_readfirstlane(u.row0);
   u.nrow = __builtin_amdgcn_readfirstlane(u.nrow);
-  if (u.chunk0 >= u.len) return;                // whole block
+  if (u.chunk0 >= u.len || u.nrow <= 0) return; // whole block
   if constexpr (PQ > 0) {
     if (!u.own) {
-      staged_unit<D, PQ, FP8>(a, u, mem);
+      staged_unit<D, PQ, FP8>(a, u, places, mem);
       return;
     }
   }
-  direct_unit<D, OQ, FP8>(a, u, mem, m_s, l_s);
+  direct_unit<D, OQ, FP8>(a, u, places, mem, m_s, l_s);
 }
 
 // One wave per query row: its group's live prefix chunks, its own live chunks, the sink.
-template <int D>
+template <int D, bool FP8>
 __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) {
   const int lane = threadIdx.x & 63;
   const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
@@ -663,8 +682,13 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
   uint16_t* dst = static_cast<uint16_t*>(a.p.out) + b * a.p.out_stride[0] + s * a.p.out_stride[1] + h * a.p.out_stride[2];
   if (sub == 0) {
-    reinterpret_cast<uint32_t*>(dst + d)[0] = pack2bf(o[0] * inv, o[1] * inv);
-    reinterpret_cast<uint32_t*>(dst + d)[1] = pack2bf(o[2] * inv, o[3] * inv);
+    if constexpr (FP8) {
+      reinterpret_cast<uint32_t*>(dst + d)[0] = pack2bf(o[0] * inv, o[1] * inv);
+      reinterpret_cast<uint32_t*>(dst + d)[1] = pack2bf(o[2] * inv, o[3] * inv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[element_of<D, FP8>(d + e)] = (uint16_t)f2bf(o[e] * inv);
+    }
   }
 }
 
@@ -709,7 +733,7 @@ void shared_run(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
     }
   }
   const long long rows = (long long)a.p.B * a.p.s_tkg * a.p.nq;
-  hipLaunchKernelGGL(attn_shared_combine_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((attn_shared_combine_kernel<D, FP8>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
 }
 
 }  // namespace

@@ -2008,10 +2008,6 @@ int mkd_attention_shared_prefix(const mkd_shared_prefix_args* a, void* workspace
   if (int rc = check_paged("attention_shared_prefix", a->k_cache, a->v_cache, a->k_cache_stride, a->v_cache_stride,
                            a->num_blocks, a->block_len, a->nkv, a->kv_format, 16))
     return rc;
-  const int eb = a->kv_format ? 1 : 2;
-  for (const long long* st : {a->k_cache_stride, a->v_cache_stride})
-    MKD_REQUIRE(((a->num_blocks - 1) * st[0] + (a->block_len - 1) * st[1] + (a->nkv - 1) * st[2] + a->d) * eb / 16 < (1LL << 32) - 1,
-                MKD_ERR_UNSUPPORTED, "attention_shared_prefix: a cache of more than 64 GiB");
   if (a->B == 0) return MKD_OK;
   const SharedPlan p = shared_plan(*a);
   MKD_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->lens && (a->tables || a->own_blocks == 0) &&
