@@ -172,6 +172,16 @@ struct Rows {
       for (int dt = 0; dt < NDT; ++dt) o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
   }
+  // After the last step: the accumulators in their registers (else the compiler brings them
+  // into the order of the stores in every step, behind each product).
+  MKD_DEV void settle() {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      asm("" : "+v"(l[t]));
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) asm("" : "+v"(o[t][dt]));
+    }
+  }
   // Raw products sc of tile t (times scale2: scores) to its P operand.  The maximum that the
   // exponentials refer to follows the largest score only where that is more than 2^8 above
   // it: the sums keep their relative precision, and the accumulators are seldom rescaled.
@@ -342,6 +352,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& plac
     if (sn < nst) load_v(sn);
   }
   // ---- merge the waves into this chunk's partial ----
+  rows.settle();
   __syncthreads();                              // the addresses are read; o_s takes their place
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -542,6 +553,7 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
          vat + (st + 2) * kShStep, un.chunk0 + st * kShStep, st + 2 < nst);
   }
   if (!live) return;
+  rows.settle();
   // ---- the wave's rows out: row 4 q4 + i of tile t, its sum from every lane column, its
   // maximum from lane column 4 q4 + i (a lane forms one row's place, the others ask it) ----
   const int n = min(un.nrow - first, 16 * QT);
