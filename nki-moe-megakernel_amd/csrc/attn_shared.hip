@@ -27,6 +27,8 @@
 // The rows' places in the caches are formed once per chunk in LDS, so blocks of any length
 // may end inside a tile; a position past the length or in no valid block is a row of zeros
 // (so that what a page holds behind a sequence, NaN among it, never meets a product).
+#include <type_traits>
+
 #include "common.h"
 #include "mkd_internal.h"
 #include "coherent.h"
@@ -172,6 +174,12 @@ struct Rows {
       for (int dt = 0; dt < NDT; ++dt) o[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
   }
+  // (kept in registers: else formed anew in front of every product)
+  static MKD_DEV u32x4_t ones() {
+    u32x4_t v = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    asm("" : "+v"(v));
+    return v;
+  }
   // After the last step: the accumulators in their registers (else the compiler brings them
   // into the order of the stores in every step, behind each product).
   MKD_DEV void settle() {
@@ -185,7 +193,7 @@ struct Rows {
   // Raw products sc of tile t (times scale2: scores) to its P operand.  The maximum that the
   // exponentials refer to follows the largest score only where that is more than 2^8 above
   // it: the sums keep their relative precision, and the accumulators are seldom rescaled.
-  MKD_DEV u32x4_t weigh(int t, const f32x4_t (&sc)[2], float scale2) {
+  MKD_DEV u32x4_t weigh(int t, const f32x4_t (&sc)[2], float scale2, u32x4_t ones) {
     const int q4 = (threadIdx.x & 63) >> 4;
     float mx = most(most(sc[0][0], sc[0][1]), sc[0][2]);
     mx = most(most(mx, sc[0][3]), sc[1][0]);
@@ -213,7 +221,7 @@ struct Rows {
       ph[2 * u] = pack2bf(p[0], p[1]);
       ph[2 * u + 1] = pack2bf(p[2], p[3]);
     }
-    l[t] = mfma16x16x32(ph, u32x4_t{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, l[t]);
+    l[t] = mfma16x16x32(ph, ones, l[t]);
     return ph;
   }
 };
@@ -292,6 +300,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& plac
       }
   };
   Rows<QT, NDT> rows;
+  const u32x4_t ones = rows.ones();
   int st = w;
   if (st < nst) {
     load_k(st);
@@ -320,7 +329,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& plac
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       if (p0 + kShStep > lim_min) hide(sc[t], p0, lim[t]);
-      ph[t] = rows.weigh(t, sc[t], scale2);
+      ph[t] = rows.weigh(t, sc[t], scale2, ones);
     }
     // P . V: lane column col owns the NDT contiguous elements of its V rows, d-tile dt is
     // element dt; the operand's 16-bit halves from two rows by one byte permute per dword
@@ -417,9 +426,13 @@ MKD_DEV void wait_loads() {                     // all but the last N vector mem
 }
 
 // ---- staged: wave w holds rows 16 QT w .., every step's K and V rows through LDS ----
-// A stage holds 32 K rows, then 32 V rows, in pieces of 16 bytes; piece p of row r is the
-// row's piece p ^ r (modulo the pieces of a row), so that the 16 rows of an operand read
-// lie on different banks.
+// A stage holds 32 K rows, then 32 V rows, in pieces of 16 bytes; the piece p of row r lies
+// at p ^ turn(r): the 8 rows of a K read's cycle on different banks (256 bytes of them), and
+// of 4 successive rows' neighbouring pieces, the transposed V reads, none on another's.
+template <int CPR>
+constexpr MKD_DEV int turn(int r) {
+  return CPR == 16 ? ((r << 1) | ((r >> 3) & 1)) & 15 : (CPR == 8 ? ((r & ~1) | ((r >> 3) & 1)) & 7 : (r >> 2) & 3);
+}
 template <int D, int QT, bool FP8>
 MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& places, char* mem) {
   constexpr int EB = FP8 ? 1 : 2, NK = D / 32, NDT = D / 16;
@@ -453,7 +466,7 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
     for (int i = 0; i < CPW; ++i) {
       const int n = w * CPW + i;
       const int piece = (n >= CPR / 2 ? n - CPR / 2 : n) * 64 + lane, row = piece / CPR, p = piece % CPR;
-      g_to_lds16((gptr)at[i] + ((p ^ (row & (CPR - 1))) << 4), dst + n * 1024);
+      g_to_lds16((gptr)at[i] + ((p ^ turn<CPR>(row)) << 4), dst + n * 1024);
     }
   };
 #pragma unroll 1
@@ -461,8 +474,9 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
   Rows<QT, NDT> rows;
   const bool live = first < un.nrow;            // (uniform)
   // operand reads: K row 16 u + col, V rows 16 u + 4 q4 + ..
-  const int kx = (col & (CPR - 1)) << 4;
-  const int vrow = 4 * q4 + (col >> 2), vx = (vrow & (CPR - 1)) << 4;
+  const int kx = turn<CPR>(col) << 4;
+  const int vrow = 4 * q4 + (col >> 2), vx = turn<CPR>(vrow) << 4;
+  const u32x4_t ones = rows.ones();
   auto step = [&](const char* __restrict ks, char* __restrict dst, const uint64_t* __restrict ka,
                   const uint64_t* __restrict va, int p0, bool more) {
     if (more) copy(dst, ka, va);
@@ -494,7 +508,7 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       if (p0 + kShStep > un.len) hide(sc[t], p0, un.len);
-      ph[t] = rows.weigh(t, sc[t], scale2);
+      ph[t] = rows.weigh(t, sc[t], scale2, ones);
     }
     if constexpr (FP8) {
       // lane column col owns NDT contiguous elements (one byte each) of its V rows
@@ -504,7 +518,7 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int row = 16 * u + 4 * q4 + j, byte = col * NDT;
-          const char* p = vs + row * RB + ((byte & ~15) ^ ((row & (CPR - 1)) << 4)) + (byte & 15);
+          const char* p = vs + row * RB + ((byte & ~15) ^ (turn<CPR>(row & 15) << 4)) + (byte & 15);
 #pragma unroll
           for (int e = 0; e < NDT / 4; ++e) vr[u][j][e] = reinterpret_cast<const uint32_t*>(p)[e];
         }
@@ -545,12 +559,20 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
       }
     }
   };
-  for (int st = 0; st < nst; ++st) {
+  // (three stages a turn: their places in LDS are constants)
+  auto turn_of = [&](int st, auto slot) {
+    constexpr int S = decltype(slot)::value;
+    if (st >= nst) return;
     if (st + 1 < nst) wait_loads<CPW>();        // stage st landed: this wave's part ..
     else wait_loads<0>();
     lds_barrier();                              // .. and everyone's; stage st - 1 is read
-    step(ring + st % kShStages * kStage, ring + (st + 2) % kShStages * kStage, kat + (st + 2) * kShStep,
-         vat + (st + 2) * kShStep, un.chunk0 + st * kShStep, st + 2 < nst);
+    step(ring + S * kStage, ring + (S + 2) % kShStages * kStage, kat + (st + 2) * kShStep, vat + (st + 2) * kShStep,
+         un.chunk0 + st * kShStep, st + 2 < nst);
+  };
+  for (int st = 0; st < nst; st += kShStages) {
+    turn_of(st, std::integral_constant<int, 0>{});
+    turn_of(st + 1, std::integral_constant<int, 1>{});
+    turn_of(st + 2, std::integral_constant<int, 2>{});
   }
   if (!live) return;
   rows.settle();
@@ -721,7 +743,7 @@ SharedPlan shared_plan(const mkd_shared_prefix_args& p) {
     return (int)(c < 128 ? 128 : (c > kShMaxChunk ? kShMaxChunk : c));
   };
   s.prefix_chunk = chunk_for(plen, s.prefix_tiles * p.nkv, 512);
-  s.own_chunk = chunk_for(olen, (long long)p.B * s.own_tiles * p.nkv, 1024);
+  s.own_chunk = chunk_for(olen, (long long)p.B * s.own_tiles * p.nkv, 512);
   s.prefix_chunks = (plen + s.prefix_chunk - 1) / s.prefix_chunk;
   s.own_chunks = (olen + s.own_chunk - 1) / s.own_chunk;
   s.prefix_units = (s.prefix_chunks * p.nkv + 7) / 8 * 8 * s.prefix_tiles;
