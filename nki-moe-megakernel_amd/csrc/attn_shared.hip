@@ -6,14 +6,15 @@
 // prefix of a group is attended once by a matrix of ALL its query rows (sequences x new
 // tokens x the kv head's query heads), each sequence's own positions by its own rows,
 // and a second launch joins a row's partials:
-//   1. units of both kinds in one grid, the prefixes' first: (chunk of positions, kv head,
-//      tile of a group's rows), and (chunk, kv head, tile of a sequence's rows)
+//   1. units of both kinds in one grid, the sequences' own first (short ones, beside which
+//      the prefixes' start): (chunk of positions, kv head, tile of a sequence's rows), and
+//      (chunk, kv head, tile of a group's rows)
 //   2. combine: one wave per row over its live chunks, the sink joined there
 //
 // Per 32-position step a wave with QT tiles of 16 query rows forms
 //   S = K . q^T   v_mfma_f32_16x16x32_bf16, A = 16 K rows, B = 16 query rows;
 //                 D lane l holds S[position 4 (l/16) + i][row l % 16]
-//   O += P . V    P straight from the S layout, V rows transposed on the way
+//   O += P . V    P straight from the S layout, V rows transposed by byte permutes
 //   l += P . 1    the sum of the same rounded P, by one more MFMA
 // P is rounded to bf16 for the matrix instruction (a relative 2^-9 of each term, the
 // rounding of the output itself); scores, maxima, l and O stay fp32.
@@ -242,10 +243,33 @@ MKD_DEV long long part_at(const SharedArgs& a, const Unit& u, int r) {   // the 
   return (((long long)(u.b0 + rr / r1) * S + (rr / gqa) % S) * a.p.nq + u.kvh * gqa + rr % gqa) * a.slots + u.slot;
 }
 
-// A partial's elements lie as a lane holds them: bf16 caches' at (d % 16) D / 16 + d / 16
-// (the transposed reads give lane column d % 16 the elements 16 apart), e4m3's at d.
-template <int D, bool FP8>
-MKD_DEV int element_of(int at) { return FP8 ? at : at % (D / 16) * 16 + at / (D / 16); }
+// The B operand of P . V for d-tile dt, element dt of the D / 16 contiguous ones that lane
+// column l % 16 holds of its 8 V rows (u, j: position 16 u + 4 (l / 16) + j).  bf16: the
+// operand's halves from two rows by one byte permute per dword (selector 0x05040100: bytes
+// 0-1 of each row; 0x07060302: bytes 2-3).
+template <bool FP8, int VD>
+MKD_DEV u32x4_t v_operand(const uint32_t (&vr)[2][4][VD], int dt) {
+  u32x4_t bop;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if constexpr (FP8) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x2_t v = (dt & 2) ? cvt2_hi(vr[u][j][dt >> 2]) : cvt2_lo(vr[u][j][dt >> 2]);
+        x[j] = v[dt & 1];
+      }
+      bop[2 * u] = pack2bf(x[0], x[1]);
+      bop[2 * u + 1] = pack2bf(x[2], x[3]);
+    } else {
+      const int e = dt >> 1;
+      const uint32_t sel = (dt & 1) ? 0x07060302u : 0x05040100u;
+      bop[2 * u] = __builtin_amdgcn_perm(vr[u][1][e], vr[u][0][e], sel);
+      bop[2 * u + 1] = __builtin_amdgcn_perm(vr[u][3][e], vr[u][2][e], sel);
+    }
+  }
+  return bop;
+}
 
 // ---- direct: position steps w, w + 4, .. to wave w, the waves merged at the end ----
 template <int D, int QT, bool FP8>
@@ -331,30 +355,9 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& plac
       if (p0 + kShStep > lim_min) hide(sc[t], p0, lim[t]);
       ph[t] = rows.weigh(t, sc[t], scale2, ones);
     }
-    // P . V: lane column col owns the NDT contiguous elements of its V rows, d-tile dt is
-    // element dt; the operand's 16-bit halves from two rows by one byte permute per dword
-    // (selector 0x05040100: bytes 0-1 of each row; 0x07060302: bytes 2-3)
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
-      u32x4_t bop;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if constexpr (FP8) {
-          float x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x2_t v = (dt & 2) ? cvt2_hi(vr[u][j][dt >> 2]) : cvt2_lo(vr[u][j][dt >> 2]);
-            x[j] = v[dt & 1];
-          }
-          bop[2 * u] = pack2bf(x[0], x[1]);
-          bop[2 * u + 1] = pack2bf(x[2], x[3]);
-        } else {
-          const int e = dt >> 1;
-          const uint32_t sel = (dt & 1) ? 0x07060302u : 0x05040100u;
-          bop[2 * u] = __builtin_amdgcn_perm(vr[u][1][e], vr[u][0][e], sel);
-          bop[2 * u + 1] = __builtin_amdgcn_perm(vr[u][3][e], vr[u][2][e], sel);
-        }
-      }
+      const u32x4_t bop = v_operand<FP8>(vr, dt);
 #pragma unroll
       for (int t = 0; t < QT; ++t) rows.o[t][dt] = mfma16x16x32(ph[t], bop, rows.o[t][dt]);
     }
@@ -388,8 +391,7 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& plac
     for (int q = 0; q < kShWaves; ++q) {
       const float f = m_s[q][r] == -INFINITY ? 0.f : exp2_hw(m_s[q][r] - M);
       L += l_s[q][r] * f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) O[e] += o_s[(q * ROWS + r) * D + element_of<D, FP8>(e0 + e)] * f;
+      O += *reinterpret_cast<const f32x4_t*>(o_s + ((q * ROWS + r) * D + e0)) * f;
     }
     const long long at = part_at(a, un, r);
     *reinterpret_cast<f32x4_t*>(a.part_o + at * D + e0) = O;
@@ -402,24 +404,6 @@ MKD_DEV void g_to_lds16(gptr src, char* dst) {   // lane l's 16 bytes to dst + 1
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                    (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
-// V operands of 4 d-tiles: out[2 i + u] from at[i] and OFF * u bytes behind it.  Per 16 lanes
-// the instruction takes a tile of 4 rows x 16 of 16-bit values, lane i naming the 8 bytes of
-// row i / 4 and columns 4 (i % 4) .., and gives lane j column j.  (Written out, with its wait:
-// after the builtin's form the compiler waits for every copy to LDS in flight.)
-template <int OFF>
-MKD_DEV void lds_tr8(uint64_t (&out)[8], const uint32_t (&at)[4]) {
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(out[0]), "=&v"(out[1]), "=&v"(out[2]), "=&v"(out[3]), "=&v"(out[4]), "=&v"(out[5]), "=&v"(out[6]),
-        "=&v"(out[7])
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFF)
-      : "memory");
-}
-MKD_DEV uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
 template <int N>
 MKD_DEV void wait_loads() {                     // all but the last N vector memory accesses
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
@@ -427,16 +411,17 @@ MKD_DEV void wait_loads() {                     // all but the last N vector mem
 
 // ---- staged: wave w holds rows 16 QT w .., every step's K and V rows through LDS ----
 // A stage holds 32 K rows, then 32 V rows, in pieces of 16 bytes; the piece p of row r lies
-// at p ^ turn(r): the 8 rows of a K read's cycle on different banks (256 bytes of them), and
-// of 4 successive rows' neighbouring pieces, the transposed V reads, none on another's.
+// at p ^ turn(r): the 8 rows that a K read takes at a time lie on different banks (256
+// bytes of them).
 template <int CPR>
 constexpr MKD_DEV int turn(int r) {
-  return CPR == 16 ? ((r << 1) | ((r >> 3) & 1)) & 15 : (CPR == 8 ? ((r & ~1) | ((r >> 3) & 1)) & 7 : (r >> 2) & 3);
+  return CPR == 16 ? r & 15 : (CPR == 8 ? (r >> 1) & 7 : (r >> 2) & 3);
 }
 template <int D, int QT, bool FP8>
 MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& places, char* mem) {
   constexpr int EB = FP8 ? 1 : 2, NK = D / 32, NDT = D / 16;
   constexpr int RB = D * EB, CPR = RB / 16;     // bytes, pieces of a row
+  constexpr int VD = RB / 64;                   // dwords of a lane's V row share
   constexpr int kStage = 2 * kShStep * RB, CPW = CPR / kShWaves;   // 1 KiB copies per wave and stage
   static_assert(CPW >= 1, "a copy per wave");
   char* const ring = mem;
@@ -473,9 +458,7 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
   for (int st = 0; st < min(nst, 2); ++st) copy(ring + st * kStage, kat + st * kShStep, vat + st * kShStep);
   Rows<QT, NDT> rows;
   const bool live = first < un.nrow;            // (uniform)
-  // operand reads: K row 16 u + col, V rows 16 u + 4 q4 + ..
   const int kx = turn<CPR>(col) << 4;
-  const int vrow = 4 * q4 + (col >> 2), vx = turn<CPR>(vrow) << 4;
   const u32x4_t ones = rows.ones();
   auto step = [&](const char* __restrict ks, char* __restrict dst, const uint64_t* __restrict ka,
                   const uint64_t* __restrict va, int p0, bool more) {
@@ -504,59 +487,34 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
         for (int kk = 0; kk < NK; ++kk) sc[t][u] = mfma16x16x32(kf[kk], qf[t][kk], sc[t][u]);
       }
     }
+    // the V rows, on their way through the softmax
+    uint32_t vr[2][4][VD];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = 16 * u + 4 * q4 + j, byte = col * (4 * VD);
+        const char* p = vs + row * RB + ((byte & ~15) ^ (turn<CPR>(row & 15) << 4)) + (byte & 15);
+        typedef uint32_t __attribute__((ext_vector_type(VD == 1 ? 2 : VD))) dwords;
+        if constexpr (VD == 1) {
+          vr[u][j][0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+          const dwords v = *reinterpret_cast<const dwords*>(p);
+#pragma unroll
+          for (int e = 0; e < VD; ++e) vr[u][j][e] = v[e];
+        }
+      }
     u32x4_t ph[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       if (p0 + kShStep > un.len) hide(sc[t], p0, un.len);
       ph[t] = rows.weigh(t, sc[t], scale2, ones);
     }
-    if constexpr (FP8) {
-      // lane column col owns NDT contiguous elements (one byte each) of its V rows
-      uint32_t vr[2][4][NDT / 4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int dt = 0; dt < NDT; ++dt) {
+      const u32x4_t bop = v_operand<FP8>(vr, dt);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = 16 * u + 4 * q4 + j, byte = col * NDT;
-          const char* p = vs + row * RB + ((byte & ~15) ^ (turn<CPR>(row & 15) << 4)) + (byte & 15);
-#pragma unroll
-          for (int e = 0; e < NDT / 4; ++e) vr[u][j][e] = reinterpret_cast<const uint32_t*>(p)[e];
-        }
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) {
-        u32x4_t bop;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x2_t v = (dt & 2) ? cvt2_hi(vr[u][j][dt >> 2]) : cvt2_lo(vr[u][j][dt >> 2]);
-            x[j] = v[dt & 1];
-          }
-          bop[2 * u] = pack2bf(x[0], x[1]);
-          bop[2 * u + 1] = pack2bf(x[2], x[3]);
-        }
-#pragma unroll
-        for (int t = 0; t < QT; ++t) rows.o[t][dt] = mfma16x16x32(ph[t], bop, rows.o[t][dt]);
-      }
-    } else {
-      // d-tile dt is the elements 16 dt + col, transposed by the read itself
-      const uint32_t base = lds_address(vs) + vrow * RB + (col & 1) * 8;
-#pragma unroll
-      for (int d0 = 0; d0 < NDT; d0 += 4) {
-        uint32_t at[4];
-        uint64_t v[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) at[i] = base + (((2 * (d0 + i) + ((col >> 1) & 1)) << 4) ^ vx);
-        lds_tr8<16 * RB>(v, at);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const u32x4_t bop = {(uint32_t)v[2 * i], (uint32_t)(v[2 * i] >> 32), (uint32_t)v[2 * i + 1],
-                               (uint32_t)(v[2 * i + 1] >> 32)};
-#pragma unroll
-          for (int t = 0; t < QT; ++t) rows.o[t][d0 + i] = mfma16x16x32(ph[t], bop, rows.o[t][d0 + i]);
-        }
-      }
+      for (int t = 0; t < QT; ++t) rows.o[t][dt] = mfma16x16x32(ph[t], bop, rows.o[t][dt]);
     }
   };
   // (three stages a turn: their places in LDS are constants)
@@ -612,7 +570,8 @@ __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArg
   int L = blockIdx.x;
   Unit u;
   Places places;
-  if (L < a.prefix_units) {
+  if (L >= a.own_units) {
+    L -= a.own_units;
     // the tiles of one (chunk, kv head) on one XCD (workgroups go round-robin by index)
     constexpr int per = PQ > 0 ? kShWaves * 16 * PQ : 16 * OQ;
     const int cell = L / (8 * a.prefix_tiles) * 8 + L % 8, tile = L / 8 % a.prefix_tiles;
@@ -639,7 +598,7 @@ __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArg
     u.kvh = cell % a.p.nkv;
     u.slot = c;
   } else {
-    L -= a.prefix_units;
+    if (L >= a.p.B * a.own_tiles * a.p.nkv * a.own_chunks) return;   // (their number is rounded up to 8)
     const int c = L % a.own_chunks, rest = L / a.own_chunks, tile = rest / a.p.nkv % a.own_tiles;
     u.own = true;
     u.kvh = rest % a.p.nkv;
@@ -668,7 +627,7 @@ __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArg
 }
 
 // One wave per query row: its group's live prefix chunks, its own live chunks, the sink.
-template <int D, bool FP8>
+template <int D>
 __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) {
   const int lane = threadIdx.x & 63;
   const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
@@ -716,13 +675,8 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
   uint16_t* dst = static_cast<uint16_t*>(a.p.out) + b * a.p.out_stride[0] + s * a.p.out_stride[1] + h * a.p.out_stride[2];
   if (sub == 0) {
-    if constexpr (FP8) {
-      reinterpret_cast<uint32_t*>(dst + d)[0] = pack2bf(o[0] * inv, o[1] * inv);
-      reinterpret_cast<uint32_t*>(dst + d)[1] = pack2bf(o[2] * inv, o[3] * inv);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dst[element_of<D, FP8>(d + e)] = (uint16_t)f2bf(o[e] * inv);
-    }
+    reinterpret_cast<uint32_t*>(dst + d)[0] = pack2bf(o[0] * inv, o[1] * inv);
+    reinterpret_cast<uint32_t*>(dst + d)[1] = pack2bf(o[2] * inv, o[3] * inv);
   }
 }
 
@@ -742,12 +696,12 @@ SharedPlan shared_plan(const mkd_shared_prefix_args& p) {
     c = (c + 127) / 128 * 128;
     return (int)(c < 128 ? 128 : (c > kShMaxChunk ? kShMaxChunk : c));
   };
-  s.prefix_chunk = chunk_for(plen, s.prefix_tiles * p.nkv, 512);
-  s.own_chunk = chunk_for(olen, (long long)p.B * s.own_tiles * p.nkv, 512);
+  s.prefix_chunk = chunk_for(plen, s.prefix_tiles * p.nkv, 256);
+  s.own_chunk = chunk_for(olen, (long long)p.B * s.own_tiles * p.nkv, 256);
   s.prefix_chunks = (plen + s.prefix_chunk - 1) / s.prefix_chunk;
   s.own_chunks = (olen + s.own_chunk - 1) / s.own_chunk;
   s.prefix_units = (s.prefix_chunks * p.nkv + 7) / 8 * 8 * s.prefix_tiles;
-  s.own_units = s.own_chunks * p.nkv * s.own_tiles * p.B;
+  s.own_units = (s.own_chunks * p.nkv * s.own_tiles * p.B + 7) / 8 * 8;
   return s;
 }
 
@@ -767,7 +721,7 @@ void shared_run(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
     }
   }
   const long long rows = (long long)a.p.B * a.p.s_tkg * a.p.nq;
-  hipLaunchKernelGGL((attn_shared_combine_kernel<D, FP8>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(attn_shared_combine_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
 }
 
 }  // namespace

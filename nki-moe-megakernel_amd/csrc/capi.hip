@@ -2024,7 +2024,7 @@ int mkd_attention_shared_prefix(const mkd_shared_prefix_args* a, void* workspace
   s.own_chunks = (int)p.own_chunks;
   s.prefix_tiles = (int)p.prefix_tiles;
   s.own_tiles = p.own_tiles;
-  s.prefix_units = (int)p.prefix_units;
+  s.own_units = (int)p.own_units;
   s.slots = (int)(p.prefix_chunks + p.own_chunks);
   const size_t parts = (size_t)a->B * a->s_tkg * a->nq * s.slots;
   Carver c{static_cast<char*>(workspace), workspace_bytes};

@@ -574,7 +574,7 @@ struct SharedPlan {
 };
 struct SharedArgs {
   mkd_shared_prefix_args p;
-  int prefix_chunk, own_chunk, prefix_chunks, own_chunks, prefix_tiles, own_tiles, prefix_units;
+  int prefix_chunk, own_chunk, prefix_chunks, own_chunks, prefix_tiles, own_tiles, own_units;
   int slots;                              // partials per row
   float *part_o, *part_ml;                // [rows][slots][d], [rows][slots][2]
 };
