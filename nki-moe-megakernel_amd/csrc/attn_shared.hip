@@ -191,39 +191,49 @@ struct Rows {
       for (int dt = 0; dt < NDT; ++dt) asm("" : "+v"(o[t][dt]));
     }
   }
-  // Raw products sc of tile t (times scale2: scores) to its P operand.  The maximum that the
+  // Raw products sc (times scale2: scores) to the tiles' P operands.  The maximum that the
   // exponentials refer to follows the largest score only where that is more than 2^8 above
   // it: the sums keep their relative precision, and the accumulators are seldom rescaled.
-  MKD_DEV u32x4_t weigh(int t, const f32x4_t (&sc)[2], float scale2, u32x4_t ones) {
+  // (One branch for all tiles, so that their chains of operations interleave.)
+  MKD_DEV void weigh(const f32x4_t (&sc)[QT][2], float scale2, u32x4_t ones, u32x4_t (&ph)[QT]) {
     const int q4 = (threadIdx.x & 63) >> 4;
-    float mx = most(most(sc[0][0], sc[0][1]), sc[0][2]);
-    mx = most(most(mx, sc[0][3]), sc[1][0]);
-    mx = quad_rows_max(most(most(most(mx, sc[1][1]), sc[1][2]), sc[1][3])) * scale2;
-    if (__any(mx > m[t] + 8.f)) {               // uniform
-      const float mn = most(m[t], mx), alpha = m[t] == -INFINITY ? 0.f : exp2_hw(m[t] - mn);
-      m[t] = mn;
-      float al[4];                              // (o and l rows are 4 q4 + i)
+    float mx[QT];
+    bool moved = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * q4 + i, 64);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) l[t][i] *= al[i];
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][dt][i] *= al[i];
+    for (int t = 0; t < QT; ++t) {
+      const f32x4_t x = sc[t][0], y = sc[t][1];
+      mx[t] = quad_rows_max(most(most(most(most(x[0], x[1]), x[2]), most(x[3], y[0])), most(most(y[1], y[2]), y[3]))) * scale2;
+      moved = moved || mx[t] > m[t] + 8.f;
     }
-    const float ms = m[t] == -INFINITY ? 0.f : -m[t];
-    u32x4_t ph;
+    if (__any(moved)) {                         // uniform
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float p[4];
+      for (int t = 0; t < QT; ++t) {
+        const float mn = most(m[t], mx[t]), alpha = m[t] == -INFINITY ? 0.f : exp2_hw(m[t] - mn);
+        m[t] = mn;
+        float al[4];                            // (o and l rows are 4 q4 + i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = exp2_hw(fmaf(sc[u][i], scale2, ms));
-      ph[2 * u] = pack2bf(p[0], p[1]);
-      ph[2 * u + 1] = pack2bf(p[2], p[3]);
+        for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * q4 + i, 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[t][i] *= al[i];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][dt][i] *= al[i];
+      }
     }
-    l[t] = mfma16x16x32(ph, ones, l[t]);
-    return ph;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float ms = m[t] == -INFINITY ? 0.f : -m[t];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = exp2_hw(fmaf(sc[t][u][i], scale2, ms));
+        ph[t][2 * u] = pack2bf(p[0], p[1]);
+        ph[t][2 * u + 1] = pack2bf(p[2], p[3]);
+      }
+      l[t] = mfma16x16x32(ph[t], ones, l[t]);
+    }
   }
 };
 // positions that row `lim` does not see
@@ -350,11 +360,10 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& plac
     }
     if (sn < nst) load_k(sn);
     u32x4_t ph[QT];
+    if (p0 + kShStep > lim_min)
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      if (p0 + kShStep > lim_min) hide(sc[t], p0, lim[t]);
-      ph[t] = rows.weigh(t, sc[t], scale2, ones);
-    }
+      for (int t = 0; t < QT; ++t) hide(sc[t], p0, lim[t]);
+    rows.weigh(sc, scale2, ones, ph);
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
       const u32x4_t bop = v_operand<FP8>(vr, dt);
@@ -505,11 +514,10 @@ MKD_DEV void staged_unit(const SharedArgs& a, const Unit& un, const Places& plac
         }
       }
     u32x4_t ph[QT];
+    if (p0 + kShStep > un.len)
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      if (p0 + kShStep > un.len) hide(sc[t], p0, un.len);
-      ph[t] = rows.weigh(t, sc[t], scale2, ones);
-    }
+      for (int t = 0; t < QT; ++t) hide(sc[t], p0, un.len);
+    rows.weigh(sc, scale2, ones, ph);
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
       const u32x4_t bop = v_operand<FP8>(vr, dt);
@@ -680,23 +688,27 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
   }
 }
 
-// Shapes alone decide the split (lengths stay on the device).
+// Shapes alone decide the split (lengths stay on the device).  Staged prefixes take 32 rows
+// per wave where that leaves every CU a unit of 512 positions (64 sequences x 8 heads x 8192
+// positions x 4 kv heads: 27.5 us, 16 rows per wave 30.7), else 16 (15 sequences x 4 tokens x
+// 4100 positions: 22.5 and 20.0 us; 6 groups of 42 x 2000: 18.1 and 14.4), two units a CU.
 SharedPlan shared_plan(const mkd_shared_prefix_args& p) {
   SharedPlan s{};
   const long long r1 = (long long)p.s_tkg * (p.nq / p.nkv), rows = r1 * p.B;
   const long long plen = p.G > 0 ? (long long)p.prefix_blocks * p.block_len : 0, olen = (long long)p.own_blocks * p.block_len;
-  s.prefix_qt = rows <= 32 ? 0 : (rows <= 64 ? 1 : 2);
+  const bool wide = (rows + 127) / 128 * p.nkv * ((plen + 511) / 512) >= 256;
+  s.prefix_qt = rows <= 32 ? 0 : (wide ? 2 : 1);
   s.own_qt = (rows <= 32 ? rows : r1) <= 16 ? 1 : 2;
   s.own_tiles = (int)((r1 + 16 * s.own_qt - 1) / (16 * s.own_qt));
   const int per = s.prefix_qt ? 16 * kShWaves * s.prefix_qt : 16 * s.own_qt;
   s.prefix_tiles = p.G > 0 ? (rows + per - 1) / per + p.G - 1 : 0;
-  auto chunk_for = [](long long len, long long units, long long want) {   // positions per block
-    long long n = units > 0 ? (want + units - 1) / units : 1;              // chunks wanted
-    long long c = (len + n - 1) / n;
-    c = (c + 127) / 128 * 128;
+  // positions per unit, in whole steps of all waves, for about `want` units
+  auto chunk_for = [](long long len, long long units, long long want) {
+    const long long n = units > 0 ? (want + units - 1) / units : 1;
+    const long long c = ((len + n - 1) / n + 127) / 128 * 128;
     return (int)(c < 128 ? 128 : (c > kShMaxChunk ? kShMaxChunk : c));
   };
-  s.prefix_chunk = chunk_for(plen, s.prefix_tiles * p.nkv, 256);
+  s.prefix_chunk = chunk_for(plen, s.prefix_tiles * p.nkv, wide ? 256 : 512);
   s.own_chunk = chunk_for(olen, (long long)p.B * s.own_tiles * p.nkv, 256);
   s.prefix_chunks = (plen + s.prefix_chunk - 1) / s.prefix_chunk;
   s.own_chunks = (olen + s.own_chunk - 1) / s.own_chunk;
