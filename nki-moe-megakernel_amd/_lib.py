@@ -91,18 +91,13 @@ KV_FP8 = 1            # MKD_KV_FP8
 KV_K_TRANSPOSED = 2   # MKD_KV_K_TRANSPOSED
 
 
-def _steps(name, n):
-    """The n strides of an array field, one field each (filled faster from Python)."""
-    return [(f"{name}{i}", i64) for i in range(n)]
-
-
 class KvAppendArgs(C.Structure):
     _fields_ = [
         ("q", vp), ("k", vp), ("v", vp), ("x_dtype", i32),
-        *_steps("q_stride", 2), *_steps("k_stride", 2), *_steps("v_stride", 2),
-        ("q_out", vp), *_steps("q_out_stride", 2), ("q_norm", vp), ("k_norm", vp), ("eps", f32),
+        ("q_stride", i64 * 2), ("k_stride", i64 * 2), ("v_stride", i64 * 2),
+        ("q_out", vp), ("q_out_stride", i64 * 2), ("q_norm", vp), ("k_norm", vp), ("eps", f32),
         ("cos", vp), ("sin", vp), ("table_rows", i32), ("rot", i32), ("positions", vp), ("positions_i64", i32),
-        ("k_cache", vp), ("v_cache", vp), *_steps("k_cache_stride", 3), *_steps("v_cache_stride", 3),
+        ("k_cache", vp), ("v_cache", vp), ("k_cache_stride", i64 * 3), ("v_cache_stride", i64 * 3),
         ("num_blocks", i32), ("block_len", i32), ("kv_format", i32), ("k_scale", vp), ("v_scale", vp),
         ("slots", vp), ("slots_i64", i32), ("T", i32), ("nq", i32), ("nkv", i32), ("d", i32),
     ]
@@ -110,8 +105,8 @@ class KvAppendArgs(C.Structure):
 
 class SharedPrefixArgs(C.Structure):
     _fields_ = [
-        ("q", vp), *_steps("q_stride", 3), ("out", vp), *_steps("out_stride", 3),
-        ("k_cache", vp), ("v_cache", vp), *_steps("k_cache_stride", 3), *_steps("v_cache_stride", 3),
+        ("q", vp), ("q_stride", i64 * 3), ("out", vp), ("out_stride", i64 * 3),
+        ("k_cache", vp), ("v_cache", vp), ("k_cache_stride", i64 * 3), ("v_cache_stride", i64 * 3),
         ("num_blocks", i32), ("block_len", i32), ("kv_format", i32),
         ("prefix_tables", vp), ("prefix_lens", vp), ("prefix_starts", vp), ("tables", vp), ("lens", vp),
         ("G", i32), ("prefix_blocks", i32), ("own_blocks", i32), ("softmax_scale", f32), ("sink", vp),
@@ -200,6 +195,7 @@ KCLASS = {"moe_gate_up": 1, "moe_down": 2, "qkv": 3, "oproj": 4, "attn": 5, "lm_
 EXPORTED = tuple(_SIGS)
 
 _lib = None
+_native = None
 
 
 def load(path: str = LIB_PATH):
@@ -248,27 +244,15 @@ def require_gpu(*tensors):
             raise ValueError("mkd operators take device (HIP) tensors; got a CPU tensor")
 
 
-def gpu_index(**tensors) -> int:
-    """The GPU that all the given tensors are on (None: absent)."""
-    dev = None
-    for name, t in tensors.items():
-        if t is not None:
-            at = t.get_device()
-            if at != dev:
-                if at < 0:
-                    raise ValueError(f"mkd operators take device (HIP) tensors; {name} is a CPU tensor")
-                if dev is not None:
-                    raise ValueError(f"{name} is on GPU {at}, the tensors before it on GPU {dev}")
-                dev = at
-    return dev
-
-
-def call(fn, what: str, index: int, *args):
-    """fn(*args, stream) on the current stream of GPU `index`, errors raised."""
-    if index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != MKD_OK:
-        check(rc, what)
+def native():
+    """The native torch boundary (csrc/torch_ops.cpp), loaded once behind libmkd.so."""
+    global _native
+    if _native is None:
+        load()
+        path = os.path.join(PKG_DIR, "_mkd_torch.so")
+        if not os.path.exists(path):
+            raise MkdLibraryMissing(f"{path} not found: build it with `python nki-moe-megakernel_amd/build.py`")
+        from . import _mkd_torch
+        _mkd_torch.set_error(MkdError)
+        _native = _mkd_torch
+    return _native

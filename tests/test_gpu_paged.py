@@ -320,3 +320,27 @@ def test_streams_and_graph(mk, dev):
         eager = step()
         assert torch.equal(out, eager), i
         torch.ones(1000, device=dev).sum().item()
+
+
+def test_in_place_refusals(mk, dev):
+    """Caches and outputs whose rows share memory or start off their boundaries, and tensors elsewhere."""
+    K, V = (torch.zeros(2, 16, 2, 128, dtype=BF, device=dev) for _ in range(2))
+    q, k, v = (torch.zeros(3, h, 128, dtype=BF, device=dev) for h in (4, 2, 2))
+    slots = torch.arange(3, device=dev)
+    shared = torch.zeros(1, 16, 2, 128, dtype=BF, device=dev).expand(2, -1, -1, -1)
+    off = torch.zeros(2 * 16 * 2 * 128 + 2, dtype=BF, device=dev)[2:].view(2, 16, 2, 128)
+    turned = torch.zeros(2, 16, 128, 2, dtype=BF, device=dev).transpose(2, 3)
+    for bad in (shared, off, turned):
+        with pytest.raises(ValueError, match="in place"):
+            mk.kv_append_rope(q, k, v, None, None, None, bad, V, slots)
+        with pytest.raises(ValueError, match="in place"):
+            mk.attention_shared_prefix(q, K, bad, None, None, None, torch.zeros(3, 1, dtype=torch.int32, device=dev),
+                                       torch.zeros(3, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError, match="in place"):
+        mk.kv_append_rope(q, k, v, None, None, None, K, V, slots, output=q[:1].expand(3, -1, -1))
+    with pytest.raises(ValueError, match="CPU tensor"):
+        mk.kv_append_rope(q, k, v, None, None, None, K, V, slots.cpu())
+    with pytest.raises(ValueError, match="CPU tensor"):
+        mk.sample_tokens(torch.zeros(2, 9, device=dev), torch.zeros(2))
+    with pytest.raises(ValueError, match="CPU tensor"):
+        mk.sample_tokens(torch.zeros(2, 9, device=dev), torch.zeros(2, device=dev), top_p=torch.ones(2))
