@@ -25,6 +25,9 @@
 // positions): the waves take steps of their own, rows straight to registers a step ahead,
 // and merge at the end: nothing to share, and no barrier to wait at.
 //
+// whole (short contexts): one direct unit takes a sequence's prefix and own positions as one
+// chunk and writes the output itself: one launch, the prefix read again per sequence.
+//
 // The rows' places in the caches are formed once per chunk in LDS, so blocks of any length
 // may end inside a tile; a position past the length or in no valid block is a row of zeros
 // (so that what a page holds behind a sequence, NaN among it, never meets a product).
@@ -59,6 +62,8 @@ MKD_DEV u32x4_t codes_to_bf16(uint32_t a, uint32_t b) {
   const f32x2_t x = cvt2_lo(a), y = cvt2_hi(a), z = cvt2_lo(b), w = cvt2_hi(b);
   return u32x4_t{pack2bf(x[0], x[1]), pack2bf(y[0], y[1]), pack2bf(z[0], z[1]), pack2bf(w[0], w[1])};
 }
+// 1 / l; a row that sees nothing (l = 0) becomes zeros, a NaN stays one
+MKD_DEV float inverse(float l) { return l > 0.f ? 1.f / l : l; }
 MKD_DEV float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The tile-th tile of `per` rows among the groups' rows (r1 rows a sequence), by one
@@ -85,6 +90,17 @@ MKD_DEV bool find_tile(const SharedArgs& a, int tile, int per, int r1, int lane,
   return false;
 }
 
+// The group of sequence b: the last one that starts at b or before it, -1 where that one
+// has ended (by every wave for itself).
+MKD_DEV int group_of(const SharedArgs& a, int b, int lane) {
+  int started = 0;
+  for (int g0 = 0; g0 <= a.p.G; g0 += 64) {
+    const int i = g0 + lane;
+    started += __popcll(__ballot(a.p.G > 0 && i <= a.p.G && a.p.prefix_starts[min(i, a.p.G)] <= b));
+  }
+  return started <= a.p.G ? started - 1 : -1;
+}
+
 }  // namespace
 
 namespace {
@@ -95,7 +111,8 @@ constexpr int kShStages = 3;                    // LDS ring of the staged form
 // positions [chunk0, min(chunk0 + CP, len)) of one table, as partial `slot`.
 struct Unit {
   int b0, row0, nrow, len, chunk0, CP, kvh, slot, width;
-  bool own;                                     // new token i sees len - (S - 1 - i) positions
+  bool own;                                     // new token i sees len - (S - 1 - i) positions ..
+  int first_own;                                // .. but the prefix in front of these always (whole units)
 };
 
 // Query rows of the unit as B operands: lane's row 16 t + col, head element 32 kk + 8 q4
@@ -117,18 +134,28 @@ MKD_DEV void load_q(const SharedArgs& a, const Unit& u, int first, u32x4_t (&qf)
       const u32x4_t v = ld16(src + (FP8 ? q4 * (D / 4) + 8 * kk : 32 * kk + 8 * q4));
       qf[t][kk] = r < u.nrow ? v ^ u32x4_t{flip, flip, flip, flip} : u32x4_t{0u, 0u, 0u, 0u};
     }
-    lim[t] = u.own ? u.len - (S - 1 - s) : u.len;
+    lim[t] = u.own ? max(u.len - (S - 1 - s), u.first_own) : u.len;
   }
 }
 // Addresses of the chunk's rows in the caches; a row of zeros for a position past the
 // length or in no valid block.  The table is read before the length is known.
 struct Places {
   int blk[kShMaxChunk / (64 * kShWaves)];
+  int front;                                    // whole units: positions of the prefix table in front
   MKD_DEV void load(const SharedArgs& a, const int* table, int width, int chunk0, int CP) {
+    front = 0;
 #pragma unroll
     for (int k = 0; k < kShMaxChunk / (64 * kShWaves); ++k) {
       const int i = threadIdx.x + 64 * kShWaves * k;
       blk[k] = i < CP ? table[min((chunk0 + i) / a.p.block_len, width - 1)] : -1;
+    }
+  }
+  MKD_DEV void load(const SharedArgs& a, const int* prefix, int plen, const int* own, int olen) {
+    front = plen;
+#pragma unroll
+    for (int k = 0; k < kShMaxChunk / (64 * kShWaves); ++k) {
+      const int i = threadIdx.x + 64 * kShWaves * k;
+      blk[k] = i < plen ? prefix[i / a.p.block_len] : (i < plen + olen ? own[(i - plen) / a.p.block_len] : -1);
     }
   }
   MKD_DEV void store(const SharedArgs& a, const Unit& u, int eb, int n, uint64_t* kat, uint64_t* vat) const {
@@ -140,7 +167,7 @@ struct Places {
       if (i >= n) break;
       const char *ka = reinterpret_cast<const char*>(g_zero_row), *va = ka;
       if (t < u.len && (unsigned)blk[k] < (unsigned)a.p.num_blocks) {
-        const int r = t % a.p.block_len;
+        const int r = (t < front ? t : t - front) % a.p.block_len;
         ka = kc + (blk[k] * a.p.k_cache_stride[0] + r * a.p.k_cache_stride[1]) * eb;
         va = vc + (blk[k] * a.p.v_cache_stride[0] + r * a.p.v_cache_stride[1]) * eb;
       }
@@ -282,7 +309,7 @@ MKD_DEV u32x4_t v_operand(const uint32_t (&vr)[2][4][VD], int dt) {
 }
 
 // ---- direct: position steps w, w + 4, .. to wave w, the waves merged at the end ----
-template <int D, int QT, bool FP8>
+template <int D, int QT, bool FP8, bool WHOLE>
 MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& places, char* mem, float (*m_s)[32],
                          float (*l_s)[32]) {
   constexpr int EB = FP8 ? 1 : 2;               // bytes per cached element
@@ -401,6 +428,20 @@ MKD_DEV void direct_unit(const SharedArgs& a, const Unit& un, const Places& plac
       const float f = m_s[q][r] == -INFINITY ? 0.f : exp2_hw(m_s[q][r] - M);
       L += l_s[q][r] * f;
       O += *reinterpret_cast<const f32x4_t*>(o_s + ((q * ROWS + r) * D + e0)) * f;
+    }
+    if constexpr (WHOLE) {
+      const int gqa = a.p.nq / a.p.nkv, rr = un.row0 + r, h = un.kvh * gqa + rr % gqa;
+      if (a.p.sink) {
+        const float sk = a.p.sink[h] * kLog2e, top = most(M, sk), f = M == -INFINITY ? 0.f : exp2_hw(M - top);
+        L = L * f + (sk == -INFINITY ? 0.f : exp2_hw(sk - top));
+        O *= f;
+      }
+      const float inv = inverse(L);
+      uint16_t* dst = static_cast<uint16_t*>(a.p.out) + un.b0 * a.p.out_stride[0] + rr / gqa % a.p.s_tkg * a.p.out_stride[1] +
+                      h * a.p.out_stride[2] + e0;
+      reinterpret_cast<uint32_t*>(dst)[0] = pack2bf(O[0] * inv, O[1] * inv);
+      reinterpret_cast<uint32_t*>(dst)[1] = pack2bf(O[2] * inv, O[3] * inv);
+      continue;
     }
     const long long at = part_at(a, un, r);
     *reinterpret_cast<f32x4_t*>(a.part_o + at * D + e0) = O;
@@ -577,6 +618,7 @@ __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArg
   const int r1 = a.p.s_tkg * (a.p.nq / a.p.nkv);
   int L = blockIdx.x;
   Unit u;
+  u.first_own = 0;
   Places places;
   if (L >= a.own_units) {
     L -= a.own_units;
@@ -631,7 +673,33 @@ __global__ void __launch_bounds__(64 * kShWaves, 2) attn_shared_kernel(SharedArg
       return;
     }
   }
-  direct_unit<D, OQ, FP8>(a, u, places, mem, m_s, l_s);
+  direct_unit<D, OQ, FP8, false>(a, u, places, mem, m_s, l_s);
+}
+
+// Short contexts: block (kv head, tile of a sequence's rows, sequence).
+template <int D, bool FP8, int OQ>
+__global__ void __launch_bounds__(64 * kShWaves, OQ == 1 ? 3 : 2) attn_shared_whole_kernel(SharedArgs a) {
+  constexpr int kTab = 2 * kShMaxChunk * 8, kOut = kShWaves * 16 * OQ * D * 4;
+  __shared__ __attribute__((aligned(1024))) char mem[kOut > kTab ? kOut : kTab];
+  __shared__ float m_s[kShWaves][32], l_s[kShWaves][32];
+  const int r1 = a.p.s_tkg * (a.p.nq / a.p.nkv);
+  Unit u;
+  u.own = true;
+  u.kvh = blockIdx.x;
+  u.row0 = blockIdx.y * 16 * OQ;
+  u.b0 = blockIdx.z;
+  u.nrow = min(r1 - u.row0, 16 * OQ);
+  u.chunk0 = u.slot = 0;
+  const int olen = min(max(a.p.lens[u.b0], 0), a.p.own_blocks * a.p.block_len);
+  const int g = __builtin_amdgcn_readfirstlane(group_of(a, u.b0, threadIdx.x & 63));
+  const int plen = g >= 0 ? min(max(a.p.prefix_lens[g], 0), a.p.prefix_blocks * a.p.block_len) : 0;
+  Places places;
+  places.load(a, a.p.prefix_tables + (long long)max(g, 0) * a.p.prefix_blocks, plen,
+              a.p.tables + (long long)u.b0 * a.p.own_blocks, olen);
+  u.len = __builtin_amdgcn_readfirstlane(plen + olen);
+  u.CP = kShMaxChunk;
+  u.first_own = plen;
+  direct_unit<D, OQ, FP8, true>(a, u, places, mem, m_s, l_s);
 }
 
 // One wave per query row: its group's live prefix chunks, its own live chunks, the sink.
@@ -641,15 +709,9 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
   const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
   if (row >= (long long)a.p.B * a.p.s_tkg * a.p.nq) return;
   const int h = (int)(row % a.p.nq), b = (int)(row / a.p.nq / a.p.s_tkg), s = (int)(row / a.p.nq % a.p.s_tkg);
-  // the group: the last one that starts at b or before
-  int started = 0;
-  for (int g0 = 0; g0 <= a.p.G; g0 += 64) {
-    const int i = g0 + lane;
-    started += __popcll(__ballot(a.p.G > 0 && i <= a.p.G && a.p.prefix_starts[min(i, a.p.G)] <= b));
-  }
+  const int g = group_of(a, b, lane);
   int np = 0;
-  if (started > 0 && started <= a.p.G)
-    np = (min(max(a.p.prefix_lens[started - 1], 0), a.p.prefix_blocks * a.p.block_len) + a.prefix_chunk - 1) / a.prefix_chunk;
+  if (g >= 0) np = (min(max(a.p.prefix_lens[g], 0), a.p.prefix_blocks * a.p.block_len) + a.prefix_chunk - 1) / a.prefix_chunk;
   const int no = (min(max(a.p.lens[b], 0), a.p.own_blocks * a.p.block_len) + a.own_chunk - 1) / a.own_chunk;
   const int n = np + no;
   const float* ml = a.part_ml + row * a.slots * 2;
@@ -680,7 +742,7 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
     for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], k, 64);
   }
   if (a.p.sink) L += exp2_hw(a.p.sink[h] * kLog2e - ms);
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  const float inv = inverse(L);
   uint16_t* dst = static_cast<uint16_t*>(a.p.out) + b * a.p.out_stride[0] + s * a.p.out_stride[1] + h * a.p.out_stride[2];
   if (sub == 0) {
     reinterpret_cast<uint32_t*>(dst + d)[0] = pack2bf(o[0] * inv, o[1] * inv);
@@ -698,7 +760,8 @@ SharedPlan shared_plan(const mkd_shared_prefix_args& p) {
   const long long plen = p.G > 0 ? (long long)p.prefix_blocks * p.block_len : 0, olen = (long long)p.own_blocks * p.block_len;
   const bool wide = (rows + 127) / 128 * p.nkv * ((plen + 511) / 512) >= 256;
   s.prefix_qt = rows <= 32 ? 0 : (wide ? 2 : 1);
-  s.own_qt = (rows <= 32 ? rows : r1) <= 16 ? 1 : 2;
+  s.whole = plen + olen <= kShMaxChunk && (r1 + 31) / 32 * p.nkv * p.B <= 512;
+  s.own_qt = (rows <= 32 && !s.whole ? rows : r1) <= 16 ? 1 : 2;
   s.own_tiles = (int)((r1 + 16 * s.own_qt - 1) / (16 * s.own_qt));
   const int per = s.prefix_qt ? 16 * kShWaves * s.prefix_qt : 16 * s.own_qt;
   s.prefix_tiles = p.G > 0 ? (rows + per - 1) / per + p.G - 1 : 0;
@@ -721,6 +784,13 @@ namespace {
 
 template <int D, bool FP8>
 void shared_run(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
+  if (p.whole) {
+    const int gqa = a.p.nq / a.p.nkv, per = 16 * p.own_qt;
+    const dim3 whole(a.p.nkv, (a.p.s_tkg * gqa + per - 1) / per, a.p.B);
+    if (p.own_qt == 1) hipLaunchKernelGGL((attn_shared_whole_kernel<D, FP8, 1>), whole, dim3(64 * kShWaves), 0, s, a);
+    else hipLaunchKernelGGL((attn_shared_whole_kernel<D, FP8, 2>), whole, dim3(64 * kShWaves), 0, s, a);
+    return;
+  }
   const dim3 grid((unsigned)(p.prefix_units + p.own_units)), block(64 * kShWaves);
   if (grid.x > 0) {
     switch (p.prefix_qt * 2 + p.own_qt) {

@@ -1995,7 +1995,7 @@ static int check_shared(const mkd_shared_prefix_args* a) {
 size_t mkd_shared_prefix_workspace_bytes(const mkd_shared_prefix_args* a) {
   if (check_shared(a)) return 0;
   const SharedPlan p = shared_plan(*a);
-  const size_t parts = (size_t)a->B * a->s_tkg * a->nq * (p.prefix_chunks + p.own_chunks);
+  const size_t parts = p.whole ? 0 : (size_t)a->B * a->s_tkg * a->nq * (p.prefix_chunks + p.own_chunks);
   Carver c{nullptr, 0};
   c.take<float>(parts * a->d);
   c.take<float>(parts * 2);
@@ -2026,7 +2026,7 @@ int mkd_attention_shared_prefix(const mkd_shared_prefix_args* a, void* workspace
   s.own_tiles = p.own_tiles;
   s.own_units = (int)p.own_units;
   s.slots = (int)(p.prefix_chunks + p.own_chunks);
-  const size_t parts = (size_t)a->B * a->s_tkg * a->nq * s.slots;
+  const size_t parts = p.whole ? 0 : (size_t)a->B * a->s_tkg * a->nq * s.slots;
   Carver c{static_cast<char*>(workspace), workspace_bytes};
   s.part_o = c.take<float>(parts * a->d);
   s.part_ml = c.take<float>(parts * 2);

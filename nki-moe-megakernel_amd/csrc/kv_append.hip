@@ -150,17 +150,28 @@ __global__ void __launch_bounds__(256) kv_append_kernel(mkd_kv_append_args a) {
 
 namespace {
 
-template <int D, bool F32, bool FP8>
+template <int D, bool F32, bool FP8, int HPT>
 void append_run(const mkd_kv_append_args& a, hipStream_t s) {
-  const long long items = (long long)a.T * (a.nq + 2 * a.nkv);
+  const long long items = (long long)a.T * ((a.nq + 2 * a.nkv + HPT - 1) / HPT);
   const unsigned blocks = (unsigned)((items + 2048 / D - 1) / (2048 / D));
-  hipLaunchKernelGGL((kv_append_kernel<D, F32, FP8, 1>), dim3(blocks), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((kv_append_kernel<D, F32, FP8, HPT>), dim3(blocks), dim3(256), 0, s, a);
+}
+// Four heads per lane group (more loads in flight, the table row read once) for bf16 grids
+// that fill the chip: 4096 tokens of 32 + 2 x 4 heads of 128 in 20.7 us instead of 23.4 (86 MB,
+// 4.2 TB/s; a copy reaches 4.85), 2047 fp32 tokens of 16 + 2 x 16 heads 17.2 instead of 15.8.
+template <int D, bool F32, bool FP8>
+void append_size(const mkd_kv_append_args& a, hipStream_t s) {
+  const long long lanes = (long long)a.T * (a.nq + 2 * a.nkv) * (D / 8);
+  if constexpr (!F32) {
+    if (lanes >= 1 << 20) return append_run<D, F32, FP8, 4>(a, s);
+  }
+  append_run<D, F32, FP8, 1>(a, s);
 }
 template <int D>
 void append_pick(const mkd_kv_append_args& a, hipStream_t s) {
   const bool f32 = a.x_dtype == MKD_DT_F32, fp8 = a.kv_format & MKD_KV_FP8;
-  if (f32) fp8 ? append_run<D, true, true>(a, s) : append_run<D, true, false>(a, s);
-  else fp8 ? append_run<D, false, true>(a, s) : append_run<D, false, false>(a, s);
+  if (f32) fp8 ? append_size<D, true, true>(a, s) : append_size<D, true, false>(a, s);
+  else fp8 ? append_size<D, false, true>(a, s) : append_size<D, false, false>(a, s);
 }
 
 }  // namespace

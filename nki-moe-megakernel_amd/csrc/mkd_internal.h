@@ -566,6 +566,7 @@ hipError_t moe_finalize_launch(const float* ybuf, int T, int K, int H, const int
 hipError_t kv_append_launch(const mkd_kv_append_args& a, hipStream_t s);
 // attn_shared.hip: how a call's positions split into blocks, from its shapes alone
 struct SharedPlan {
+  bool whole;                             // one launch, prefix and own positions of a sequence together
   int prefix_qt, own_qt;                  // 16-row tiles per wave of staged prefixes (0: direct), of direct units
   int own_tiles;                          // tiles of one sequence's rows
   long long prefix_tiles;                 // tiles of all groups' rows, at most
