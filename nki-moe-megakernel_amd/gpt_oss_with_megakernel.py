@@ -34,6 +34,7 @@ from . import _lib as L
 from . import packing
 from .qwen_with_megakernel import (EXPERT_FORMATS, _LayerStack, _prefill, check_waits, pack_experts_mx,
                                    randn_bf16, tensor_seed)
+from .sample import sample_tokens
 
 VARIANT_GPT_OSS = 1
 
@@ -314,8 +315,9 @@ class GptOssMegakernelModel(_LayerStack, nn.Module):
         L.check(rc, "gpt_oss decode_layers")
         return hidden
 
-    def step(self, token_ids, position_ids, hidden, logits, next_tokens):
-        """Greedy decode step into caller buffers (no allocation; graph-capturable)."""
+    def step(self, token_ids, position_ids, hidden, logits, next_tokens, sampling: Optional[dict] = None):
+        """Decode step into caller buffers (graph-capturable): greedy without an allocation, or
+        with `sampling` (sample_tokens' arguments beside the logits) drawn from the logits."""
         lib = L.load()
         B = hidden.shape[0]
         Hp = self.cfg.hidden_pad
@@ -328,6 +330,8 @@ class GptOssMegakernelModel(_LayerStack, nn.Module):
                                        self.cfg.hidden_size, 1, logits.data_ptr(),
                                        next_tokens.data_ptr(), self.lm_ws.data_ptr(),
                                        self.lm_ws.numel(), s), "lm_head")
+        if sampling is not None:
+            sample_tokens(logits, output=next_tokens, **sampling)
         return next_tokens
 
     def prefill(self, input_ids: torch.Tensor, start_pos: int = 0, seq: int = 0, chunk: int = 4096):

@@ -29,6 +29,7 @@ from torch import nn
 
 from . import _lib as L
 from . import packing
+from .sample import sample_tokens
 
 
 def set_decode_path(mode: str = "multi_kernel") -> None:
@@ -447,8 +448,10 @@ class Qwen3MoeMegakernelModel(_LayerStack, nn.Module):
         return hidden
 
     def step(self, token_ids: torch.Tensor, position_ids: torch.Tensor, hidden: torch.Tensor,
-             logits: torch.Tensor, next_tokens: torch.Tensor):
-        """Full greedy decode step into caller buffers (no allocation; graph-capturable)."""
+             logits: torch.Tensor, next_tokens: torch.Tensor, sampling: Optional[dict] = None):
+        """Full decode step into caller buffers (graph-capturable).  Greedy without an
+        allocation; with `sampling` (sample_tokens' arguments: uniforms [B], and any of
+        temperature, top_k, top_p, min_p) next_tokens are drawn from the logits instead."""
         lib = L.load()
         B, H = hidden.shape
         s = L.stream_ptr(self.device)
@@ -459,6 +462,8 @@ class Qwen3MoeMegakernelModel(_LayerStack, nn.Module):
                                        self.lm_head_packed.data_ptr(), B, H, self.cfg.vocab_size, H, 2,
                                        logits.data_ptr(), next_tokens.data_ptr(),
                                        self.lm_ws.data_ptr(), self.lm_ws.numel(), s), "lm_head")
+        if sampling is not None:
+            sample_tokens(logits, output=next_tokens, **sampling)
         return next_tokens
 
     def prefill(self, input_ids: torch.Tensor, start_pos: int = 0, seq: int = 0, chunk: int = 4096):
@@ -471,8 +476,9 @@ class Qwen3MoeMegakernelModel(_LayerStack, nn.Module):
         return _prefill(self, input_ids, start_pos, seq, chunk, self.cfg.hidden_size,
                         self.cfg.hidden_size, 2, lambda pos: (None, None))
 
-    def forward(self, input_ids: torch.Tensor, position_ids: torch.Tensor):
-        """Greedy decode step: input_ids [B] -> (logits [B, V] fp32, next ids [B] int32).
+    def forward(self, input_ids: torch.Tensor, position_ids: torch.Tensor, sampling: Optional[dict] = None):
+        """Decode step, greedy or with `sampling` as in `step`: input_ids [B] -> (logits
+        [B, V] fp32, next ids [B] int32).
         Synchronises and raises RuntimeError when an in-launch wait of the step ran
         out (the step's results are then invalid); `step` is the graph-capturable
         form without that check."""
@@ -481,7 +487,7 @@ class Qwen3MoeMegakernelModel(_LayerStack, nn.Module):
         logits = torch.empty(B, self.cfg.vocab_size, dtype=torch.float32, device=self.device)
         nxt = torch.empty(B, dtype=torch.int32, device=self.device)
         self.step(input_ids.to(torch.int32).contiguous(), position_ids.to(torch.int32).contiguous(),
-                  hidden, logits, nxt)
+                  hidden, logits, nxt, sampling)
         check_waits(self, B, self.ws)
         return logits, nxt
 

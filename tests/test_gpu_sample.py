@@ -21,7 +21,8 @@ def check(mk, dev, logits, u, **kw):
     assert np.array_equal(tok, want), [(b, int(tok[b]), int(want[b])) for b in np.flatnonzero(tok != want)[:5]]
     none = want < 0
     assert np.array_equal(lp[none], wlp[none])
-    assert (np.abs(lp - wlp)[~none] <= 2.0 ** -24 * np.abs(wlp[~none]) + 2.0 ** -36).all()
+    lp, wlp = lp[~none], wlp[~none]
+    assert (np.abs(lp - wlp) <= 2.0 ** -24 * np.abs(wlp) + 2.0 ** -36).all()
     return tok
 
 

@@ -178,8 +178,8 @@ def test_attention_c_entry_refuses(L):
     for kw in (dict(q=None), dict(out=None), dict(lens=None), dict(tables=None), dict(prefix_tables=None), dict(prefix_starts=None)):
         assert c_attend(L, **kw) == L.MKD_ERR_NULL, kw
     assert c_attend(L, d=96) == L.MKD_ERR_UNSUPPORTED
-    assert c_attend(L, ws_bytes=64) == L.MKD_ERR_WORKSPACE
-    assert c_attend(L, ws=None, ws_bytes=0) == L.MKD_ERR_WORKSPACE
+    assert c_attend(L, ws_bytes=64, prefix_blocks=200) == L.MKD_ERR_WORKSPACE     # (short contexts need none)
+    assert c_attend(L, ws=None, ws_bytes=0, prefix_blocks=200) == L.MKD_ERR_WORKSPACE
     assert L.load().mkd_attention_shared_prefix(None, P, 0, None) == L.MKD_ERR_NULL
     assert c_attend(L, B=0, ws_bytes=0) == L.MKD_OK
 
