@@ -54,7 +54,7 @@ MKD_DEV SmSetting setting_of(const mkd_sample_args& a, int b) {
   SmSetting s;
   const float t = a.temperature_rows ? a.temperature_rows[b] : a.temperature;
   const bool greedy = !(t > 0.f);               // as top_k = 1
-  s.inv_t = greedy ? 1.0 : 1.0 / (double)t;
+  s.inv_t = greedy ? 1.0 : 1.0 / fmin((double)t, 0x1p127);   // (an infinite t: all the same, but never 0 * -inf)
   s.top_k = greedy ? 1 : (a.top_k_rows ? a.top_k_rows[b] : a.top_k);
   s.top_p = a.top_p_rows ? a.top_p_rows[b] : a.top_p;
   s.min_p = a.min_p_rows ? a.min_p_rows[b] : a.min_p;

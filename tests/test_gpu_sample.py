@@ -109,6 +109,20 @@ def test_not_finite(mk, dev):
         assert tok[0] == -1 and tok[1] == -1 and tok[3] == 4321 and tok[4] in (70, 4200)
 
 
+def test_infinite_temperature(mk, dev):
+    """Tensors of temperatures may hold an infinity: all logits but -inf and NaN weigh the same."""
+    x, u = rows(14, 8, 9000)
+    x[:, ::3] = -INF
+    x[:, 7::5] = float("nan")
+    x[1, [4, 8500]] = INF
+    for kw in (dict(), dict(top_k=700), dict(top_p=0.3), dict(top_k=9000, top_p=0.9, min_p=0.2)):
+        tok, lp = mk.sample_tokens(x.to(dev), u.to(dev), temperature=torch.full((8,), INF, device=dev),
+                                   **kw)
+        want, wlp = O.sample_tokens(x, u, temperature=2.0 ** 127, **kw)
+        assert np.array_equal(tok.cpu().numpy(), want), kw
+        assert np.abs(lp.double().cpu().numpy() - wlp).max() <= 2.0 ** -24 * np.abs(wlp).max() + 2.0 ** -36
+
+
 def test_strides_and_output(mk, dev):
     x, u = rows(10, 5, 3001)
     want, _ = O.sample_tokens(x, u, top_p=0.9)
