@@ -614,8 +614,10 @@ int mkd_kv_append_rope(const mkd_kv_append_args* args, void* stream);
  * Scores, sums and the accumulation are fp32; the probabilities enter the
  * matrix instructions as bf16.  FP8 caches are attended as stored (fold a
  * scale into softmax_scale and the output).  The cached positions of a prefix
- * are read once for all rows of a tile (up to 64 query rows of one kv head),
- * not once per sequence.  Workspace: mkd_shared_prefix_workspace_bytes(args)
+ * are read once for all rows of a tile (16, 32, 64 or 128 query rows of one kv head),
+ * not once per sequence; where the tables hold at most 1024 positions together
+ * and there are few sequences, one launch reads them per sequence instead and
+ * needs no workspace.  Workspace: mkd_shared_prefix_workspace_bytes(args)
  * (depends on the shapes alone); calls that share it must not overlap. */
 typedef struct {
   const void* q;

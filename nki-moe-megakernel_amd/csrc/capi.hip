@@ -1945,7 +1945,7 @@ static int check_paged(const char* what, const void* k, const void* v, const lon
 int mkd_kv_append_rope(const mkd_kv_append_args* a, void* stream) {
   if (int rc = stale_check("mkd_kv_append_rope")) return rc;
   MKD_REQUIRE(a, MKD_ERR_NULL, "kv_append_rope: null pointer");
-  MKD_REQUIRE(a->T >= 0 && a->nq > 0 && a->nkv > 0 && (long long)a->T * (a->nq + 2LL * a->nkv) < (1LL << 31),
+  MKD_REQUIRE(a->T >= 0 && a->nq > 0 && a->nkv > 0 && (long long)a->T * (a->nq + 2LL * a->nkv) < (1LL << 28),
               MKD_ERR_INVALID, "kv_append_rope: %d tokens of %d + 2 x %d heads", a->T, a->nq, a->nkv);
   MKD_REQUIRE(a->d == 64 || a->d == 128, MKD_ERR_UNSUPPORTED, "kv_append_rope: d %d (64 or 128)", a->d);
   MKD_REQUIRE(a->x_dtype == MKD_DT_F32 || a->x_dtype == MKD_DT_BF16, MKD_ERR_INVALID, "kv_append_rope: x_dtype %d",
@@ -1987,7 +1987,8 @@ static int check_shared(const mkd_shared_prefix_args* a) {
               MKD_ERR_INVALID, "attention_shared_prefix: %d groups of %d blocks, %d own blocks of %d rows", a->G,
               a->prefix_blocks, a->own_blocks, a->block_len);
   const SharedPlan p = shared_plan(*a);
-  MKD_REQUIRE(p.prefix_units + p.own_units < (1LL << 31) && (long long)a->B * a->s_tkg * a->nq < (1LL << 31),
+  // (2^32 threads a launch)
+  MKD_REQUIRE(p.prefix_units + p.own_units < (1LL << 24) && (long long)a->B * a->s_tkg * a->nq <= (1LL << 25),
               MKD_ERR_UNSUPPORTED, "attention_shared_prefix: %lld units of work for one call", p.prefix_units + p.own_units);
   return MKD_OK;
 }

@@ -147,7 +147,7 @@ PyObject* kv_append_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t T = q.size(0), nq = q.size(1), d = q.size(2);
   const Caches c = caches(K, V, d);
   TORCH_CHECK_VALUE(c.nkv == k.size(1), "the caches hold ", c.nkv, " kv heads, k and v ", k.size(1));
-  TORCH_CHECK_VALUE(nq >= 1 && T * (nq + 2 * c.nkv) < (1LL << 31), T, " tokens of ", nq, " + 2 x ", c.nkv, " heads");
+  TORCH_CHECK_VALUE(nq >= 1 && T * (nq + 2 * c.nkv) < (1LL << 28), T, " tokens of ", nq, " + 2 x ", c.nkv, " heads");
   const auto type = q.scalar_type();
   TORCH_CHECK_VALUE((type == at::kBFloat16 || type == at::kFloat) && k.scalar_type() == type && v.scalar_type() == type,
                     "q, k and v must all be bfloat16 or float32, got ", shape_of(q), ", ", shape_of(k), ", ", shape_of(v));
@@ -183,6 +183,7 @@ PyObject* kv_append_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
                            {"v_scale", &vs}, {"output", &out}});
   written(K, "K_cache", 4);
   written(V, "V_cache", 4);
+  TORCH_CHECK_VALUE(T == 0 || ptr(K) != ptr(V), "K_cache and V_cache are used in place and must not be one tensor");
   if (out.defined()) written(out, "output", 4);
   else out = out_tensor(q.sizes(), at::kBFloat16, q);
   if (T > 0) {

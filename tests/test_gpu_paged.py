@@ -128,9 +128,11 @@ def test_append_not_finite(mk, dev):
             assert r[0].isnan() and r[1] == (240 if fp8 else float("inf")) and r[2] == -r[1]
 
 
-def build(seed, dev, B, S, nq, nkv, d, block, fp8, sizes, first, prefix, lens, joint=False, sink=False, spoil=True):
+def build(seed, dev, B, S, nq, nkv, d, block, fp8, sizes, first, prefix, lens, joint=False, sink=False, spoil=True,
+          room=(0, 0), scale=None):
     """One attention case: (arguments on the GPU, float64 output, its weighted mean of |v|).  Rows behind
-    every length hold NaN, and unused table entries name no block."""
+    every length hold NaN, and unused table entries name no block.  room: positions that the prefix and the own
+    tables have at least (above 1024 together, the keys are split over chunks)."""
     g = torch.Generator().manual_seed(seed)
     need = [(-(-n // block)) for n in prefix + lens]
     blocks = sum(need) + 2
@@ -147,14 +149,15 @@ def build(seed, dev, B, S, nq, nkv, d, block, fp8, sizes, first, prefix, lens, j
                 V[t[i, n // block], n % block:] = float("nan")
         return t
 
-    pt = paged(prefix, max([-(-n // block) for n in prefix], default=0) + 1)
-    ot = paged(lens, max(-(-n // block) for n in lens))
+    wide = [-(-n // block) for n in room]
+    pt = paged(prefix, max([-(-n // block) for n in prefix] + [wide[0] - 1]) + 1 if prefix else 0)
+    ot = paged(lens, max([-(-n // block) for n in lens] + wide[1:]))
     if spoil:
         K[perm], V[perm] = float("nan"), float("nan")
     starts = torch.tensor([first] + [first + sum(sizes[:i + 1]) for i in range(len(sizes))], dtype=torch.int32)
     q = rand(g, B, S, nq, d, std=1.5).to(BF)
     sk = rand(g, nq) if sink else None
-    scale = d ** -0.5 / (8 if fp8 else 1)
+    scale = d ** -0.5 / (8 if fp8 else 1) if scale is None else scale
     pl, ln = torch.tensor(prefix, dtype=torch.int32), torch.tensor(lens, dtype=torch.int32)
     want = O.attention_shared_prefix(q, K, V, pt, pl, starts, ot, ln, scale, sk)
     if joint:
@@ -197,6 +200,69 @@ def test_attention_matches_float64(mk, dev, B, S, nq, nkv, d, block, fp8, sizes,
     got = mk.attention_shared_prefix(*args, **kw)
     torch.cuda.synchronize()
     assert got.shape == args[0].shape
+    check_attention(got, want)
+
+
+# The keys split over chunks: tables with room for more than 1024 positions.  The query rows of a kv head that a
+# group may have, and of one sequence, say which kernel reads the prefixes (to 32: direct; staged above, in tiles
+# of 64, or of 128 for many units) and how wide the own tiles are.
+SPLIT = [
+    # B S nq nkv block sizes first prefix lens joint sink room
+    (4, 1, 8, 2, 16, [3], 1, [333], [200, 1, 33, 0], False, True, (1100, 0)),                   # 16 rows, direct
+    (3, 2, 15, 3, 7, [1, 2], 0, [129, 500], [2, 131, 300], True, False, (0, 2000)),             # 30 rows, direct
+    (11, 3, 10, 2, 24, [4, 0, 5], 1, [260, 3, 128], [5, 1, 3, 2, 700, 40, 0, 129, 128, 31, 33], False, True, (600, 800)),
+    (9, 8, 10, 1, 1, [9], 0, [1300], [8 + 19 * i for i in range(9)], False, False, (0, 0)),     # 80 rows a sequence
+    (21, 1, 112, 16, 32, [1, 18, 2], 0, [0, 1100, 77], [1 + 13 * i for i in range(21)], True, True, (4200, 300)),
+    (10, 4, 64, 8, 16, [10], 0, [1030], [4 + 30 * i for i in range(10)], False, False, (6000, 0)),  # tiles of 128, 32 rows a sequence
+]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B,S,nq,nkv,block,sizes,first,prefix,lens,joint,sink,room", SPLIT)
+def test_attention_split_matches_float64(mk, dev, B, S, nq, nkv, block, sizes, first, prefix, lens, joint, sink, room, d, fp8):
+    print(f"split B={B} S={S} nq={nq} nkv={nkv} d={d} block={block} fp8={fp8} {sizes} {prefix} {lens}", flush=True)
+    args, kw, want = build(3 * B + d, dev, B, S, nq, nkv, d, block, fp8, sizes, first, prefix, lens, joint, sink, room=room)
+    assert (args[3].shape[1] + args[6].shape[1]) * block > 1024
+    got = mk.attention_shared_prefix(*args, **kw)
+    torch.cuda.synchronize()
+    check_attention(got, want)
+
+
+@pytest.mark.parametrize("room", [0, 1500])
+@pytest.mark.parametrize("groups", [64, 65, 150])
+def test_attention_many_groups(mk, dev, groups, room):
+    """More groups than one look at them takes, the first and the last sequences in none, some groups empty."""
+    g = torch.Generator().manual_seed(groups)
+    sizes = torch.randint(0, 3, (groups,), generator=g).tolist()
+    sizes[-1], sizes[-2] = 2, 0
+    prefix = torch.randint(0, 60, (groups,), generator=g).tolist()
+    B = sum(sizes) + 3
+    lens = torch.randint(0, 30, (B,), generator=g).tolist()
+    args, kw, want = build(groups, dev, B, 1, 6, 2, 64, 8, False, sizes, 2, prefix, lens, room=(room, 0))
+    check_attention(mk.attention_shared_prefix(*args, **kw), want)
+
+
+@pytest.mark.parametrize("room", [(0, 0), (1200, 0)])
+@pytest.mark.parametrize("B", [2, 9])
+def test_attention_scales(mk, dev, B, room):
+    """A scale of zero (the mean of the values), a negative one, and scores so far apart that one key is left."""
+    for scale in (0.0, -0.09, 3.0):
+        args, kw, want = build(B, dev, B, 2, 8, 2, 128, 16, False, [B], 0, [150], [1 + 9 * i for i in range(B)], room=room,
+                               scale=scale)
+        check_attention(mk.attention_shared_prefix(*args, **kw), want)
+
+
+@pytest.mark.parametrize("room", [(0, 0), (1200, 0)])
+@pytest.mark.parametrize("B", [3, 20])
+def test_attention_nan_query(mk, dev, B, room):
+    """A NaN or an infinity in one sequence's query stays with its row."""
+    args, kw, want = build(B, dev, B, 1, 8, 2, 64, 16, False, [B - 1], 0, [99], [1 + 5 * i for i in range(B)], room=room)
+    args[0][1, 0, 5, 3] = float("nan")
+    args[0][1, 0, 6, 4] = float("inf")
+    got = mk.attention_shared_prefix(*args, **kw).cpu()
+    assert got[1, 0, 5].isnan().all() and not got[1, 0, 6].isfinite().all()
+    got[1, 0, 5:7] = want[0][1, 0, 5:7].to(BF)
     check_attention(got, want)
 
 
@@ -338,6 +404,8 @@ def test_in_place_refusals(mk, dev):
                                        torch.zeros(3, dtype=torch.int32, device=dev))
     with pytest.raises(ValueError, match="in place"):
         mk.kv_append_rope(q, k, v, None, None, None, K, V, slots, output=q[:1].expand(3, -1, -1))
+    with pytest.raises(ValueError, match="one tensor"):
+        mk.kv_append_rope(q, k, v, None, None, None, K, K, slots)
     with pytest.raises(ValueError, match="CPU tensor"):
         mk.kv_append_rope(q, k, v, None, None, None, K, V, slots.cpu())
     with pytest.raises(ValueError, match="CPU tensor"):
