@@ -34,7 +34,8 @@ constexpr double kSmRes = 16.0;                 // bins per unit of z
 constexpr int kSmMaxChunks = (1 << 20) / kSmChunk;
 constexpr int kSmRow = 512;                     // threads of a row's block: a bin each
 constexpr int kSmStage = 8192;                  // members of a bin held in LDS
-constexpr int kSmMassBits = 50;                 // a chunk's bin: count above, mass (4096 weights) below
+constexpr int kSmRankBit = 18;                  // of the upper word
+constexpr int kSmMassBits = 32 + kSmRankBit;                 // a chunk's bin: count above, mass (4096 weights) below
 constexpr double kSmOne = 0x1p36;               // weight of the middle of a bin; at its edges 3 % off
 
 // What stage 1 leaves per (row, chunk).
@@ -47,14 +48,15 @@ struct SmRecord {
 };
 
 struct SmSetting {
-  double inv_t, top_p, min_p, u;
+  double t, inv_t, top_p, min_p, u;
   int top_k;
 };
 MKD_DEV SmSetting setting_of(const mkd_sample_args& a, int b) {
   SmSetting s;
   const float t = a.temperature_rows ? a.temperature_rows[b] : a.temperature;
   const bool greedy = !(t > 0.f);               // as top_k = 1
-  s.inv_t = greedy ? 1.0 : 1.0 / fmin((double)t, 0x1p127);   // (an infinite t: all the same, but never 0 * -inf)
+  s.t = greedy ? 1.0 : fmin((double)t, 0x1p127);   // (an infinite t: all the same, but never 0 * -inf)
+  s.inv_t = 1.0 / s.t;
   s.top_k = greedy ? 1 : (a.top_k_rows ? a.top_k_rows[b] : a.top_k);
   s.top_p = a.top_p_rows ? a.top_p_rows[b] : a.top_p;
   s.min_p = a.min_p_rows ? a.min_p_rows[b] : a.min_p;
@@ -69,21 +71,24 @@ MKD_DEV double mass_of(float l, float top, double inv_t) {
   if (top == INFINITY) return 0.0;
   return exp(((double)l - (double)top) * inv_t);
 }
-// z in bins; its whole part is the bin's place (monotone in l)
-MKD_DEV double scaled(float l, double inv_t) { return (double)l * (inv_t * kSmRes); }
-MKD_DEV double place_of(float l, double inv_t) { return floor(scaled(l, inv_t)); }
-// A token's weight from its fraction f of a bin: exp((f - 1/2) / 16), whose series to the
-// fifth power (written out in powers of f) leaves 2^-39; + 2^52 rounds to a whole number.
-constexpr double sm_term(int k) {
-  double sum = 0.0, term = 1.0;                 // term: 1 / (16^m m!)
-  for (int m = 0; m <= 5; ++m) {
-    if (m > 0) term /= kSmRes * m;
-    if (m < k) continue;
-    double c = term;                            // times binomial(m, k) (-1/2)^(m - k)
-    for (int i = 0; i < m - k; ++i) c *= -0.5 * (m - i) / (i + 1);
-    sum += c;
+// z in bins: the nearest whole number is the bin's place (monotone in l), the rest the
+// token's fraction f of a bin, -1/2 to 1/2.  Adding kSmWhole rounds the exact product.
+constexpr double kSmWhole = 0x1.8p52;
+struct SmPlace { double place, f; };
+MKD_DEV SmPlace place_of(float l, double inv_t) {
+  const double c = inv_t * kSmRes, x = l, z = x * c;
+  if (fabs(z) < 0x1p51) {
+    const double place = fma(x, c, kSmWhole) - kSmWhole;
+    return {place, fma(x, c, -place)};
   }
-  return sum * kSmOne;
+  return {rint(z), z - rint(z)};                // (-inf: a NaN fraction, used by none)
+}
+// A token's weight from its fraction: exp(f / 16), whose series to the fifth power leaves
+// 2^-39; + 2^52 rounds to a whole number.
+constexpr double sm_term(int k) {
+  double term = kSmOne;
+  for (int m = 1; m <= k; ++m) term /= kSmRes * m;
+  return term;
 }
 struct SmSeries {                               // the coefficients, in scalar registers
   double c[6];
@@ -94,11 +99,16 @@ struct SmSeries {                               // the coefficients, in scalar r
       asm("" : "+s"(c[k]));                     // (else every use moves two literals first)
     }
   }
-  MKD_DEV u64 weight(double f) const {
+  MKD_DEV u64 bits(double f) const {            // of 2^52 + the weight
     double p = c[5];
 #pragma unroll
     for (int k = 4; k >= 0; --k) p = fma(p, f, c[k]);
-    return __double_as_longlong(p) & ((1ull << 52) - 1);
+    return __double_as_longlong(p);
+  }
+  MKD_DEV u64 weight(double f) const { return bits(f) & ((1ull << 52) - 1); }
+  MKD_DEV u64 counted(double f) const {         // count << kSmMassBits | weight, by one 32-bit addition
+    const u64 b = bits(f);
+    return (u64)((uint32_t)(b >> 32) + ((1u << (kSmMassBits - 32)) - 0x43300000u)) << 32 | (uint32_t)b;
   }
 };
 // bit patterns in the order of the logits (a bf16 one's upper half); -0 and +0 are one value
@@ -166,24 +176,32 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
   for (int q = 0; q < kSmThreads / 64; ++q) top = fmaxf(top, wtop[q]);
   if (x == 0) r.top = top;
   if (top == -INFINITY) return;                 // nothing to choose here (the rest is not read)
-  const double top_place = place_of(top, s.inv_t);
-  uint16_t bin[kSmPer];
-  uint32_t rank[kSmPer];                        // among its members
-  if (top < INFINITY) {
-    const SmSeries series;
+  const double top_place = place_of(top, s.inv_t).place;
+  uint32_t at[kSmPer];                          // rank among the bin's members << kSmRankBit | bin
+  const uint32_t outside = kSmBins + (x & 31);
+  // Places of 30 bits, and what lies over 900 bins below the maximum raised to there: the
+  // distance is then a difference of the low words.
+  const float floor_l = (float)((top_place - 1024.0) * (s.t / kSmRes));
+  const SmSeries series;
+  auto put = [&](uint32_t bin, u64 one) {
+    return ((uint32_t)(atomicAdd(&bins[bin], one) >> 32) & ~((1u << kSmRankBit) - 1)) | bin;
+  };
+  if (top < INFINITY && fabs(top_place) < 0x1p30 && floor_l > -3.402823466e38f) {
+    const double c = s.inv_t * kSmRes;
+    const uint32_t top_low = (uint32_t)__double_as_longlong(top_place + kSmWhole);
 #pragma unroll
     for (int i = 0; i < kSmPer; ++i) {
-      const double z = scaled(l[i], s.inv_t), place = floor(z);
-      const double below = top_place - place;   // (-inf: infinitely far)
-      const int j = (int)below;
-      bin[i] = (uint16_t)(j < kSmBins ? j : kSmBins + (x & 31));
-      rank[i] = (uint32_t)(atomicAdd(&bins[bin[i]], (1ull << kSmMassBits) | series.weight(z - place)) >> 32);
+      const double v = fmaxf(l[i], floor_l), t = fma(v, c, kSmWhole);
+      at[i] = put(min(top_low - (uint32_t)__double_as_longlong(t), outside), series.counted(fma(v, c, -(t - kSmWhole))));
+    }
+  } else if (top < INFINITY) {
+    for (int i = 0; i < kSmPer; ++i) {
+      const SmPlace z = place_of(l[i], s.inv_t);
+      const double below = top_place - z.place; // (-inf: infinitely far)
+      at[i] = below < kSmBins ? put((uint32_t)below, series.counted(z.f)) : outside;
     }
   } else {                                      // infinite logits share the mass
-    for (int i = 0; i < kSmPer; ++i) {
-      bin[i] = l[i] == top ? 0 : kSmBins;
-      if (bin[i] < kSmBins) rank[i] = (uint32_t)(atomicAdd(&bins[0], (1ull << kSmMassBits) | (u64)kSmOne) >> 32);
-    }
+    for (int i = 0; i < kSmPer; ++i) at[i] = l[i] == top ? put(0u, (1ull << kSmMassBits) | (u64)kSmOne) : outside;
   }
   __syncthreads();
   // exclusive scan of the counts, a bin a thread
@@ -210,9 +228,10 @@ __global__ void __launch_bounds__(kSmThreads) sample_chunk_kernel(mkd_sample_arg
   r.bins[x] = mine;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kSmPer; ++i)
-    if (bin[i] < kSmBins)
-      list[first[bin[i]] + (rank[i] >> (kSmMassBits - 32))] = (uint16_t)(G * x + G * kSmThreads * (i / G) + i % G);
+  for (int i = 0; i < kSmPer; ++i) {
+    const uint32_t j = at[i] & ((1u << kSmRankBit) - 1);
+    if (j < kSmBins) list[first[j] + (at[i] >> kSmRankBit)] = (uint16_t)(G * x + G * kSmThreads * (i / G) + i % G);
+  }
   __syncthreads();
   for (unsigned i = x * 8; i < total; i += kSmThreads * 8) st16(r.list + i, ld16(list + i));
 }
@@ -347,8 +366,7 @@ struct SmRow {
 
   MKD_DEV u64 weight(uint32_t key) const {
     if (top == INFINITY) return (u64)kSmOne;
-    const double z = scaled(logit_of<BF>(key), inv_t);
-    return series.weight(z - floor(z));
+    return series.weight(place_of(logit_of<BF>(key), inv_t).f);
   }
   // member m of the staged bin: its index, and its logit's bit pattern
   MKD_DEV void member(unsigned m, uint32_t& key, uint32_t& index) const {
@@ -609,9 +627,10 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     }
     return;
   }
-  const double top_place = place_of(top, set.inv_t);
+  const SmPlace top_at = place_of(top, set.inv_t);
+  const double top_place = top_at.place;
   if (x < nc) {
-    const double d = mine == top ? 0.0 : top_place - place_of(mine, set.inv_t);
+    const double d = mine == top ? 0.0 : top_place - place_of(mine, set.inv_t).place;
     s.shift[x] = d < kSmBins ? (int)d : kSmBins;
   }
   __syncthreads();
@@ -637,7 +656,7 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
     }
     // exp(middle - z_max)
     const double unit = top == INFINITY ? 1.0 / kSmOne
-        : exp(((top_place - scaled(top, set.inv_t)) + (0.5 - x)) / kSmRes) / kSmOne;
+        : exp((-top_at.f - x) / kSmRes) / kSmOne;
     double sm = (double)m * unit;
     scan_nm(s, s.wave_d, sn, sm);
     s.cum_n[x] = sn;
@@ -661,7 +680,7 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
   if (!by_k) {
     far = last;
     if (set.min_p > 0.0 && top != INFINITY)     // one bin to spare
-      far = (int)fmin(floor(((double)top * set.inv_t - log(set.min_p)) * kSmRes - top_place) + 1.0, (double)last);
+      far = (int)fmin(floor(-log(set.min_p) * kSmRes - top_at.f) + 2.0, (double)last);
     if (by_p || !(set.min_p > 0.0)) {
       const double most = (by_p ? set.top_p : set.u) * all;
       const int j = find_bin([&](int i) { return by_p ? s.cum[i] >= most : s.cum[i] > most; });
@@ -726,7 +745,7 @@ __global__ void __launch_bounds__(kSmRow) sample_row_kernel(mkd_sample_args a, c
       cut = logit_of<BF>(k);
     }
     const uint32_t key = key_of<BF>(cut);
-    const double below = cut == top ? 0.0 : top_place - place_of(cut, set.inv_t);
+    const double below = cut == top ? 0.0 : top_place - place_of(cut, set.inv_t).place;
     if (token_of(key, 0xffffffffu) < end.token && below < kSmBins) {
       const int j = (int)below;
       row.stage(j);                             // the weight of the bin's members at least as large
