@@ -35,7 +35,7 @@ constexpr int kSmMaxChunks = (1 << 20) / kSmChunk;
 constexpr int kSmRow = 512;                     // threads of a row's block: a bin each
 constexpr int kSmStage = 8192;                  // members of a bin held in LDS
 constexpr int kSmRankBit = 18;                  // of the upper word
-constexpr int kSmMassBits = 32 + kSmRankBit;                 // a chunk's bin: count above, mass (4096 weights) below
+constexpr int kSmMassBits = 32 + kSmRankBit;    // a chunk's bin: count above, mass (8192 weights) below
 constexpr double kSmOne = 0x1p36;               // weight of the middle of a bin; at its edges 3 % off
 
 // What stage 1 leaves per (row, chunk).
