@@ -615,7 +615,7 @@ int mkd_kv_append_rope(const mkd_kv_append_args* args, void* stream);
  * matrix instructions as bf16.  FP8 caches are attended as stored (fold a
  * scale into softmax_scale and the output).  The cached positions of a prefix
  * are read once for all rows of a tile (16, 32, 64 or 128 query rows of one kv head),
- * not once per sequence; where the tables hold at most 1024 positions together
+ * not once per sequence; where a sequence's tables hold at most 1024 positions
  * and there are few sequences, one launch reads them per sequence instead and
  * needs no workspace.  Workspace: mkd_shared_prefix_workspace_bytes(args)
  * (depends on the shapes alone); calls that share it must not overlap. */

@@ -25,8 +25,19 @@
 // positions): the waves take steps of their own, rows straight to registers a step ahead,
 // and merge at the end: nothing to share, and no barrier to wait at.
 //
+// What bounds it (64 sequences, 32 heads over 4 kv heads of 128, prefix 8192, own 512:
+// 52 MB, 8.9 GFLOP): the units take 26.7 us, 2.0 TB/s and 0.33 PFLOP/s, the join 6.1 us (19
+// MB of partials written and read).  A prefix unit is 16 steps of 1820 cycles, in which a
+// wave issues 34 MFMAs, 16 16-byte LDS reads a lane, 16 exponentials, 32 byte permutes; with
+// one wave of each kind per SIMD these follow one another more than they overlap.  Without
+// the copies a step takes 8 % less, without the exponentials 13, without Q . K 11, without
+// P . V 14; K rows read two steps ahead and scores formed one step ahead gave 2 %, a ring of
+// four stages nothing.  FP8 rows (32 sequences, prefix 32768): 42.6 us, 2015 cycles a step,
+// the conversions to bf16 in place of half the copies.
+//
 // whole (short contexts): one direct unit takes a sequence's prefix and own positions as one
-// chunk and writes the output itself: one launch, the prefix read again per sequence.
+// chunk and writes the output itself: one launch, the prefix read again per sequence (2
+// sequences of 40 + 17 positions 5.0 us, by chunks and a join 9.7; the rule at shared_plan).
 //
 // The rows' places in the caches are formed once per chunk in LDS, so blocks of any length
 // may end inside a tile; a position past the length or in no valid block is a row of zeros
@@ -702,7 +713,9 @@ __global__ void __launch_bounds__(64 * kShWaves, OQ == 1 ? 3 : 2) attn_shared_wh
   direct_unit<D, OQ, FP8, true>(a, u, places, mem, m_s, l_s);
 }
 
-// One wave per query row: its group's live prefix chunks, its own live chunks, the sink.
+// One wave per query row: its group's live prefix chunks, its own live chunks, the sink.  Bound
+// by the partials' bytes (2048 rows x 17 of 520 bytes: 6.1 us, 1920 x 9: 5.1); loads that do not
+// wait for the lengths made it no faster.
 template <int D>
 __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) {
   const int lane = threadIdx.x & 63;
@@ -754,13 +767,24 @@ __global__ void __launch_bounds__(256) attn_shared_combine_kernel(SharedArgs a) 
 // per wave where that leaves every CU a unit of 512 positions (64 sequences x 8 heads x 8192
 // positions x 4 kv heads: 27.5 us, 16 rows per wave 30.7), else 16 (15 sequences x 4 tokens x
 // 4100 positions: 22.5 and 20.0 us; 6 groups of 42 x 2000: 18.1 and 14.4), two units a CU.
+// Direct to 32 rows: 8 rows x 32768 positions 21.7 us, staged 25.2; 32 rows 24.0 and 26.3
+// (at 2000 positions 11.6 and 10.9).
+// One launch for short contexts (us with it, and with chunks and a join; 4 kv heads of 128, 8
+// heads each): a block per sequence and kv head goes through its positions alone, so long
+// contexts want many blocks, and each reads the prefix anew, so many want short ones.
+//   positions   4 blocks    64 blocks   128 blocks  512 blocks   1024 blocks
+//   128         4.9   7.8   5.1   8.8   5.1   9.2    6.7  14.9   12.4  22.3
+//   512         8.5   9.0   8.6  11.1   8.7  11.8   13.4  20.3   23.2  27.8
+//   768        10.8   9.5  10.9  11.7  11.0  13.0   17.9  23.4   32.0  29.2
+//   1024       13.1   8.8  13.4  11.3  13.4  12.8   22.5  24.9   40.8  30.5
 SharedPlan shared_plan(const mkd_shared_prefix_args& p) {
   SharedPlan s{};
   const long long r1 = (long long)p.s_tkg * (p.nq / p.nkv), rows = r1 * p.B;
   const long long plen = p.G > 0 ? (long long)p.prefix_blocks * p.block_len : 0, olen = (long long)p.own_blocks * p.block_len;
   const bool wide = (rows + 127) / 128 * p.nkv * ((plen + 511) / 512) >= 256;
   s.prefix_qt = rows <= 32 ? 0 : (wide ? 2 : 1);
-  s.whole = plen + olen <= kShMaxChunk && (r1 + 31) / 32 * p.nkv * p.B <= 512;
+  const long long whole = (r1 + 31) / 32 * p.nkv * p.B, len = plen + olen;
+  s.whole = len <= 512 ? whole <= 1024 : len <= kShMaxChunk && whole <= 512 && (len <= 768 || whole >= 128);
   s.own_qt = (rows <= 32 && !s.whole ? rows : r1) <= 16 ? 1 : 2;
   s.own_tiles = (int)((r1 + 16 * s.own_qt - 1) / (16 * s.own_qt));
   const int per = s.prefix_qt ? 16 * kShWaves * s.prefix_qt : 16 * s.own_qt;

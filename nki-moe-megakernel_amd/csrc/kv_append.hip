@@ -8,7 +8,9 @@
 // D / 8 lanes per head.  Lane j < r / 8 holds the elements 4j .. 4j + 3 and their
 // partners 4j + r/2 ..: the rotation stays inside the lane; the lanes behind hold the 8
 // contiguous elements of the part that is not rotated.  The norm's sum is a DPP sum over
-// the head's lanes.  Bound by its bytes, and by the call itself at decode batches.
+// the head's lanes.  Bound by its bytes for prompts (figures at append_size), by the launch at
+// decode batches: one token of 32 + 2 x 4 heads of 128 3.5 us, 61 of 64 + 2 x 8 of 64 into an
+// FP8 cache 3.8; a call takes 6 us with its host side.
 #include "common.h"
 #include "fp8.h"
 #include "mkd_internal.h"

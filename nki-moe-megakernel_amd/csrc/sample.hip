@@ -20,6 +20,15 @@
 // temperature in fp64, as an integer of 36 bits (the bin's unit, exp(middle - z_max), joins
 // in fp64 per bin): sums of a bin are exact, whatever the order of atomic additions, and
 // its relative precision does not depend on how far below the maximum it lies.
+//
+// What it takes: chunks 6.1 us for one fp32 row of 151,936 logits, 19.7 for 64 (39 MB), 36.4
+// for 128 bf16 rows of 201,088 (51 MB read, 64 written: 3.2 TB/s).  A block is a chain of
+// loads, maximum, atomics, scan and stores, four of them on a CU; without the series 6 us
+// less of the 36, without the lists 4, without the atomics 3; blocks of 16384 logits 40 us.
+// rows 10.6 us for one row and 16 for 64, a chain of memory latencies and barriers; 38 for
+// the 128 rows, whose two searches gather the logits of some 3000 members of a bin each (a
+// memory line a logit: as much as all logits).  Both bins gathered together 37 to 42, the row
+// read again in place of the lists 66.
 #include "common.h"
 #include "mkd_internal.h"
 

@@ -190,6 +190,8 @@ CASES = [
     (70, 1, 2, 1, 64, 16, False, [70], 0, [97], [1 + i % 40 for i in range(70)], False, False),   # tiles past one
     (3, 1, 24, 1, 128, 64, True, [3], 0, [1100], [700, 64, 1], False, True),                  # 24 heads a kv head
     (2, 2, 4, 4, 128, 16, False, [], 0, [], [77, 2], False, False),                          # no groups
+    (32, 1, 8, 4, 64, 64, False, [30], 1, [830], [1 + 2 * i for i in range(32)], False, True),   # 960 positions, 128 blocks of work
+    (33, 2, 32, 4, 128, 32, True, [20, 13], 0, [860, 600], [2 + 3 * i for i in range(33)], True, False),
 ]
 
 
@@ -223,7 +225,7 @@ SPLIT = [
 def test_attention_split_matches_float64(mk, dev, B, S, nq, nkv, block, sizes, first, prefix, lens, joint, sink, room, d, fp8):
     print(f"split B={B} S={S} nq={nq} nkv={nkv} d={d} block={block} fp8={fp8} {sizes} {prefix} {lens}", flush=True)
     args, kw, want = build(3 * B + d, dev, B, S, nq, nkv, d, block, fp8, sizes, first, prefix, lens, joint, sink, room=room)
-    assert (args[3].shape[1] + args[6].shape[1]) * block > 1024
+    assert (args[3].shape[1] + args[6].shape[1]) * block > 1024      # (to there one launch may take the whole context)
     got = mk.attention_shared_prefix(*args, **kw)
     torch.cuda.synchronize()
     check_attention(got, want)
