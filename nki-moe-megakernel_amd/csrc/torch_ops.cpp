@@ -351,6 +351,7 @@ Tensor setting(PyObject* o, const char* name, int64_t B, double lo, double hi, a
   if (!THPVariable_Check(o)) {
     *value = number(o, name);
     TORCH_CHECK_VALUE(*value >= lo && *value <= hi, name, " must be in [", lo, ", ", hi, "], got ", *value);   // (a NaN too)
+    TORCH_CHECK_VALUE(type != at::kInt || *value == std::floor(*value), name, " must be a whole number, got ", *value);
     return Tensor();
   }
   const Tensor t = THPVariable_Unpack(o);

@@ -115,6 +115,7 @@ SAMPLE = [
     (dict(temperature=Z(3)), ValueError, "temperature"),
     (dict(temperature=Z(2, dtype=I32)), ValueError, "temperature"),
     (dict(top_k=-1), ValueError, "top_k"),
+    (dict(top_k=2.5), ValueError, "whole number"),
     (dict(top_k=Z(2)), ValueError, "top_k"),
     (dict(top_p=1.01), ValueError, "top_p"),
     (dict(min_p=2), ValueError, "min_p"),
