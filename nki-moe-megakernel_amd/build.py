@@ -63,7 +63,7 @@ def _link_torch(obj: str) -> None:
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = TORCH_LIB_PATH + ".tmp"
     cmd = ["g++", "-shared", "-fPIC", obj, "-o", tmp, "-L", PKG_DIR, "-l:libmkd.so", "-Wl,-rpath,$ORIGIN", "-L", libs,
-           "-lc10", "-ltorch_cpu", "-ltorch_python", "-lc10_hip"]
+           "-lc10", "-ltorch_cpu", "-ltorch_python", "-lc10_hip", "-ltorch_hip"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link of _mkd_torch.so failed:\n{r.stderr[-6000:]}")
